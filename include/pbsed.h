@@ -311,8 +311,8 @@ int pbsed_gru_set_poll_delays(int kind, int fwd, int fwd_gate, int bwd, int bwd_
  * dispatcher's placement once per device with a probe launch (XCC_ID per workgroup; the exchange stays off on any device
  * where block ids equal mod 8 do not share an XCD, or fewer than 8 XCDs answer), and every workgroup of such a ring
  * re-checks its own XCC_ID at launch: a mismatch sets bit 1 (value 2) of the scan's err_flag (bit 0 = a hand-off timed
- * out).  on = 0 switches the exchange off for the process (callers do on seeing bit 1; PBSED_GRU_XCD_LOCAL=0 does the
- * same from the environment), on = 1 allows it again.  Returns the previous setting.  Replaces nothing in the reference
+ * out).  OFF by default (placement on MI355X was seen to change between launches); on = 1 (or PBSED_GRU_XCD_LOCAL=1 in the
+ * environment) allows it, on = 0 switches it off again (callers do on seeing bit 1).  Returns the previous setting.  Replaces nothing in the reference
  * (torch.nn.GRU has no such knob: pb_sed/models/weak_label/crnn.py:61-67). */
 int pbsed_gru_set_xcd_local(int on);
 /* Diagnostics of the persistent scans: the scans launched after this call write shader-clock stamps of workgroup `block`

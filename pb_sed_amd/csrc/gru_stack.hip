@@ -992,7 +992,10 @@ int pbsed_gru_stack_fwd(int nchains, int nlayers, const float* const* gi0, const
 __global__ void xcc_probe_kernel(unsigned* out) {
     if (threadIdx.x == 0) out[blockIdx.x] = xcc_id();
 }
-static std::atomic<int> g_xcd_local_allowed{1};       // pbsed_gru_set_xcd_local (any host thread may call it beside a launching one)
+// Off unless asked for (pbsed_gru_set_xcd_local(1), or PBSED_GRU_XCD_LOCAL=1): on MI355X the dispatcher's placement is NOT the same
+// function of the block id in every launch once other kernels have run between the probe and the scan - the scans' own check saw
+// rings spread over XCDs there, whose exchange through one L2 is wrong.  (Any host thread may call the setter beside a launching one.)
+static std::atomic<int> g_xcd_local_allowed{getenv("PBSED_GRU_XCD_LOCAL") && getenv("PBSED_GRU_XCD_LOCAL")[0] == '1' ? 1 : 0};
 static std::mutex g_xcd_mu;                           // the probe's per-device verdicts below
 static int g_xcd_state[64] = {0};                     // per device ordinal: 0 not probed, 1 verified, -1 refused
 static bool xcd_placement(hipStream_t s, unsigned* map) {
@@ -1309,7 +1312,7 @@ int pbsed_gru_set_prof(unsigned long long* buf, int block) {
 }
 
 // The XCD-local exchange of the BPTT scans (GruStackArgs::local): on = 0 switches it off for the process (every ring then
-// exchanges through write-through stores and sc1 loads, correct under any workgroup placement), on = 1 allows it again where
+// exchanges through write-through stores and sc1 loads, correct under any workgroup placement), on = 1 allows it where
 // the placement probe (run anew) verifies the device.  The caller turns it off when a scan reports error bit 2.  Returns the old value.
 int pbsed_gru_set_xcd_local(int on) {
     const int old = g_xcd_local_allowed.exchange(on != 0, std::memory_order_relaxed);
