@@ -82,12 +82,12 @@ __global__ __launch_bounds__(256) void boundariesfilt_kernel(const float* __rest
     const int n = n_row[row], h = n / 2;
     for (int t = threadIdx.x; t < T; t += blockDim.x) {
         if (n > 0) {
+            // product and sum rounded one after the other, as the reference's float64 correlation rounds them (a contracted fma
+            // differs in the last bit)
+#pragma clang fp contract(off)
             const double w = 1.0 / (double)h;
             double f = 0.0, r = 0.0;
-            // valid correlation of the padded row; product and sum rounded one after the other, as the reference's float64
-            // correlation rounds them (a contracted fma differs in the last bit)
-#pragma clang fp contract(off)
-            for (int k = 0; k < n; ++k) {
+            for (int k = 0; k < n; ++k) {                        // valid correlation of the padded row
                 const int i = t + k - h;
                 const double c = (k < h) ? -w : w;
                 const double xf = (i >= 0 && i < T) ? (double)x[i] : 0.0;
