@@ -432,6 +432,67 @@ int pbsed_boundariesfilt(const float* in, float* out, double* out64, const int* 
 int pbsed_event_frames(const float* scores, const float* thr, const int* len, int* events, int* counts, int R, int T,
                        int max_events, void* stream);
 
+/* ---- state-space sequence layers (the recurrent part of pb_sed/models/weak_label/crnn.py:61-67 as a selective scan instead of a
+ * GRU; padertorch has no such layer - new in the build).  Activations are time-major [T][B][channels] in one of three element types
+ * (`dtype`), unit stride over channels, strides over frames and clips in elements; parameters, states and parameter gradients are
+ * float.  seq_len [B] or NULL (= T): frames behind it are not read and their outputs are 0; `reverse` != 0 scans a clip's valid
+ * frames from the last to the first.  Parameter gradients are ADDED to their buffers (any may be NULL), in a fixed order: results
+ * are reproducible.  Workspaces are the caller's, used only by the launches of the call. */
+#define PBSED_F32 0
+#define PBSED_BF16 1
+#define PBSED_F16 2
+/* y = act(bias + sum_j w[d][j] x[s-(K-1)+j]), 2 <= K <= 8, act = silu or identity; state [B][K-1][D] (element type, oldest first) stands in
+ * front of the first frame (NULL: zeros), state_out receives the last K-1 positions (NULL: not wanted; must not overlap state).
+ * y [T][B][D] contiguous. */
+int pbsed_causal_conv_fwd(const void* x, const float* w, const float* bias, const int* seq_len, const void* state, void* y,
+                          void* state_out, int T, int B, int D, int K, long long x_stride_t, long long x_stride_b, int silu,
+                          int reverse, int dtype, void* stream);
+long long pbsed_causal_conv_workspace(int T, int B, int D, int K);     /* floats, for dw / db */
+/* dstate_out [B][K-1][D]: gradient of state_out, or NULL; dstate: gradient of state, or NULL. */
+int pbsed_causal_conv_bwd(const void* dy, const void* x, const float* w, const float* bias, const int* seq_len, const void* state,
+                          const void* dstate_out, void* dx, void* dstate, float* dw, float* db, float* ws, long long ws_floats,
+                          int T, int B, int D, int K, long long dy_stride_t, long long dy_stride_b, long long x_stride_t,
+                          long long x_stride_b, long long dx_stride_t, long long dx_stride_b, int silu, int reverse, int dtype,
+                          void* stream);
+/* one frame: x [B][D] at a clip stride; state_out may be state. */
+int pbsed_causal_conv_step(const void* x, const float* w, const float* bias, const void* state, void* state_out, void* y, int B,
+                           int D, int K, long long x_stride_b, int silu, int dtype, void* stream);
+/* h_t = exp(D_t A) h_{t-1} + D_t u_t B_t, y_t = (C_t . h_t + skip u_t) silu(z_t) with D_t = softplus(delta_t + delta_bias) (softplus = 0: the
+ * sum itself), A = -exp(a_log [D][N]), N <= 64; b, c [T][B][N]; skip, z, delta_bias may be NULL; state / state_out [B][D][N] float or
+ * NULL.  strides (host): frame and clip stride of u, delta, b, c, z.  saved: what the backward pass needs (pbsed_selective_scan_plan
+ * gives its size), or NULL.  y [T][B][D] contiguous. */
+int pbsed_selective_scan_plan(int T, int B, int D, int N, int backward, long long* saved_floats /*host*/, long long* ws_floats /*host*/);
+int pbsed_selective_scan_fwd(const void* u, const void* delta, const float* a_log, const void* b, const void* c, const float* skip,
+                             const void* z, const float* delta_bias, const int* seq_len, const float* state, void* y, float* state_out,
+                             float* saved, float* ws, long long ws_floats, const long long* strides /*host*/, int T, int B, int D,
+                             int N, int softplus, int reverse, int dtype, void* stream);
+/* du, ddelta [T][B][D], db, dc [T][B][N] contiguous; dz at its strides; dstate_out / dstate: gradients of state_out / state or NULL.
+ * strides (host): u, delta, b, c, z, dy, dz. */
+int pbsed_selective_scan_bwd(const void* dy, const void* u, const void* delta, const float* a_log, const void* b, const void* c,
+                             const float* skip, const void* z, const float* delta_bias, const int* seq_len, const float* saved,
+                             const float* dstate_out, void* du, void* ddelta, void* db, void* dc, void* dz, float* dstate,
+                             float* da_log, float* dskip, float* ddelta_bias, float* ws, long long ws_floats,
+                             const long long* strides /*host*/, int T, int B, int D, int N, int softplus, int reverse, int dtype,
+                             void* stream);
+/* one frame: u, delta, z [B][D], b, c [B][N] at clip strides (host, in this order with z last); state_out may be state. */
+int pbsed_selective_scan_step(const void* u, const void* delta, const float* a_log, const void* b, const void* c, const float* skip,
+                              const void* z, const float* delta_bias, const float* state, float* state_out, void* y,
+                              const long long* strides /*host*/, int B, int D, int N, int softplus, int dtype, void* stream);
+/* Layer norm over the last axis of x [rows][C] (row stride x_stride): y = (x - mean) (var + eps)^-1/2 w + b; w, b may be NULL (1, 0);
+ * stats [rows][2] = mean, (var + eps)^-1/2 for the backward pass, or NULL.  y, dx contiguous. */
+int pbsed_layer_norm_fwd(const void* x, const float* w, const float* b, void* y, float* stats, long long rows, long long C,
+                         long long x_stride, float eps, int dtype, void* stream);
+long long pbsed_layer_norm_workspace(long long rows, long long C);     /* floats, for dw / db */
+int pbsed_layer_norm_bwd(const void* dy, const void* x, const float* w, const float* stats, void* dx, float* dw, float* db, float* ws,
+                         long long ws_floats, long long rows, long long C, long long dy_stride, long long x_stride, int dtype,
+                         void* stream);
+/* y[i] = [residual[i] +] (word(i) >= p 2^32 ? x[i] / (1 - p) : 0), i = row-major index in [rows][C], word(i) from Philox-4x32 with seven
+ * rounds under (i >> 2, step, site) and the key seed; rng (device) = seed, step.  The backward pass is the same call on dy.  y may be x
+ * or residual. */
+int pbsed_dropout(const void* x, const void* residual, void* y, long long rows, long long C, long long x_stride,
+                  long long residual_stride, long long y_stride, int dtype, double p, const long long* rng /*device*/, int site,
+                  void* stream);
+
 /* ---- optimiser (padertorch Adam(lr, gradient_clipping); pb_sed/experiments/weak_label_crnn/training.py:264-269) */
 int pbsed_grad_sumsq(const float* g, size_t n, double* out, void* stream);
 /* skip_flags [n_flags] (or NULL): device error words of this step's persistent GRU scans (their `err` argument); if

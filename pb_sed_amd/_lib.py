@@ -17,7 +17,8 @@ _i = C.POINTER(C.c_int)
 _u8 = C.POINTER(C.c_ubyte)
 _v = C.c_void_p
 _pp = C.POINTER(C.c_void_p)
-I, F32, F64, SZ = C.c_int, C.c_float, C.c_double, C.c_size_t
+I, F32, F64, SZ, LL = C.c_int, C.c_float, C.c_double, C.c_size_t, C.c_longlong
+_ll = C.POINTER(C.c_longlong)
 
 # name -> argtypes (all return int status unless listed in _NON_STATUS)
 SIGNATURES = {
@@ -107,6 +108,18 @@ SIGNATURES = {
     'pbsed_set_launch_cus': [I],
     'pbsed_scratch_bytes': [],
     'pbsed_memset_async': [_v, I, SZ, _v],
+    'pbsed_causal_conv_fwd': [_v] * 7 + [I, I, I, I, LL, LL, I, I, I, _v],
+    'pbsed_causal_conv_workspace': [I, I, I, I],
+    'pbsed_causal_conv_bwd': [_v] * 12 + [LL, I, I, I, I] + [LL] * 6 + [I, I, I, _v],
+    'pbsed_causal_conv_step': [_v] * 6 + [I, I, I, LL, I, I, _v],
+    'pbsed_selective_scan_plan': [I, I, I, I, I, _ll, _ll],
+    'pbsed_selective_scan_fwd': [_v] * 14 + [LL, _ll] + [I] * 7 + [_v],
+    'pbsed_selective_scan_bwd': [_v] * 22 + [LL, _ll] + [I] * 7 + [_v],
+    'pbsed_selective_scan_step': [_v] * 11 + [_ll] + [I] * 5 + [_v],
+    'pbsed_layer_norm_fwd': [_v] * 5 + [LL, LL, LL, F32, I, _v],
+    'pbsed_layer_norm_workspace': [LL, LL],
+    'pbsed_layer_norm_bwd': [_v] * 8 + [LL] * 5 + [I, _v],
+    'pbsed_dropout': [_v] * 3 + [LL] * 5 + [I, F64, _v, I, _v],
     'pbsed_comm_id_bytes': [],
     'pbsed_comm_unique_id': [_v],
     'pbsed_comm_create': [_v, I, I, _pp],
@@ -114,7 +127,7 @@ SIGNATURES = {
     'pbsed_allreduce_begin': [_v, _v, SZ, _v],
     'pbsed_allreduce_finish': [_v, _v],
 }
-_NON_STATUS = {'pbsed_gru_granule_capacity': C.c_int, 'pbsed_set_launch_cus': C.c_int, 'pbsed_gru_set_xcd_local': C.c_int, 'pbsed_conv_bwd_weight_bng_supported': C.c_int, 'pbsed_scratch_bytes': C.c_size_t, 'pbsed_last_error': C.c_char_p, 'pbsed_version': C.c_int, 'pbsed_comm_id_bytes': C.c_int, 'pbsed_conv_pack_dims': None,
+_NON_STATUS = {'pbsed_causal_conv_workspace': C.c_longlong, 'pbsed_layer_norm_workspace': C.c_longlong, 'pbsed_gru_granule_capacity': C.c_int, 'pbsed_set_launch_cus': C.c_int, 'pbsed_gru_set_xcd_local': C.c_int, 'pbsed_conv_bwd_weight_bng_supported': C.c_int, 'pbsed_scratch_bytes': C.c_size_t, 'pbsed_last_error': C.c_char_p, 'pbsed_version': C.c_int, 'pbsed_comm_id_bytes': C.c_int, 'pbsed_conv_pack_dims': None,
                'pbsed_conv_pack_dims_bf16': None, 'pbsed_conv_pack_dims_wino': None, 'pbsed_conv_pack_dims_winox3': None, 'pbsed_conv_pack_dims_s16': None,
                'pbsed_conv1d_pack_dims_x3': None}
 

@@ -7,7 +7,7 @@ HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p build
 pids=()
-for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm misc logmel postproc collective; do
+for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm causal_conv selective_scan layer_norm dropout misc logmel postproc collective; do
   if [ ! -f build/$f.o ] || [ -n "$(find $f.hip build.sh *.h *.inc -newer build/$f.o)" ]; then
     $HIPCC $FLAGS -c $f.hip -o build/$f.o &
     pids+=($!)

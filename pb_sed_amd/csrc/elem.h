@@ -1,0 +1,86 @@
+// Element types of the sequence operators (causal_conv.hip, selective_scan.hip, layer_norm.hip, dropout.hip): activations are
+// float, bfloat16 or half in memory; every computation is float; one rounding (to nearest even) at the store.
+#pragma once
+#include "common.h"
+
+namespace pbsed {
+
+enum { PBSED_DT_F32 = 0, PBSED_DT_BF16 = 1, PBSED_DT_F16 = 2 };
+
+template <class S, int V> struct alignas(sizeof(S) * V) Pack { S v[V]; };
+
+template <class S, int V>
+__device__ __forceinline__ void load_pack(const S* p, float (&out)[V]) {
+    const Pack<S, V> w = *reinterpret_cast<const Pack<S, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)w.v[i];
+}
+template <class S, int V>
+__device__ __forceinline__ void store_pack(S* p, const float (&in)[V]) {
+    Pack<S, V> w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w.v[i] = (S)in[i];
+    *reinterpret_cast<Pack<S, V>*>(p) = w;
+}
+
+__device__ __forceinline__ float fast_sigmoid(float x) {           // v_exp_f32 + v_rcp_f32: 1 ulp each
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
+}
+// exp(-x), 0 <= x <= 100, to 2 ulp: the rounding of x log2(e), which v_exp_f32 would turn into an error of x ulp, is carried along
+__device__ __forceinline__ float exp_neg(float x) {
+    const float t = -1.44269504f * x;
+    const float l = fmaf(x, -1.92596299e-8f, fmaf(x, -1.44269504f, -t));      // log2(e) = 1.44269504 (as float) + 1.92596299e-8
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, l * 0.69314718f, e);
+}
+// log(1 + exp(x)) without cancellation: max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], and log1p(e) = 2 atanh(s) with
+// s = e / (2 + e) <= 1/3 as its Taylor series in s^2 <= 1/9 (the first term left out is 9^-8 / 17 of the sum: below 2^-29)
+__device__ __forceinline__ float softplus(float x) {
+    const float e = exp_neg(fminf(fabsf(x), 100.f));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float p = 1.f / 15.f;
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    const float y = fmaf(2.f * s, p, fmaxf(x, 0.f));
+    return x != x ? x : y;                                          // v_max_f32 would drop a NaN
+}
+
+// out[i] += sum over p < P of ws[p][i]: the last step of a reduction whose blocks have left one row of partial sums each, in a fixed
+// order (results do not depend on the order in which the blocks ran); partials are added in double.  A segment = one output.
+struct SumSegs { float* out[3]; int end[3]; };                      // out may be null; end: first index behind the segment
+// grid ceil(W / 16), 256 threads: 16 columns x 16 groups of rows
+__device__ __forceinline__ void sum_partials(const float* ws, int P, long W, const SumSegs& sg, int col0, double* red) {
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const long col = col0 + c;
+    double acc = 0.;
+    if (col < W)
+        for (int p = g; p < P; p += 16) acc += (double)ws[(long)p * W + col];
+    red[g * 17 + c] = acc;
+    __syncthreads();
+    if (g == 0 && col < W) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) acc += red[k * 17 + c];
+        int s = 0;
+        while (s < 2 && col >= sg.end[s]) ++s;
+        float* o = sg.out[s];
+        if (o) {
+            o += col - (s ? sg.end[s - 1] : 0);
+            *o = (float)((double)*o + acc);
+        }
+    }
+}
+
+}  // namespace pbsed
+
+// dispatch on an element type: EXPR sees S
+#define PBSED_ELEM(dtype, ...)                                       \
+    do {                                                             \
+        if ((dtype) == pbsed::PBSED_DT_F32) { using S = float; __VA_ARGS__; }         \
+        else if ((dtype) == pbsed::PBSED_DT_BF16) { using S = __bf16; __VA_ARGS__; }  \
+        else { using S = _Float16; __VA_ARGS__; }                    \
+    } while (0)

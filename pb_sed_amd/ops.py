@@ -1320,3 +1320,384 @@ def event_frames(scores, thresholds, lengths, max_events=None):
     th_dev, ln_dev = host_to_device(th, x.device, torch.float32), host_to_device(ln, x.device, torch.int32)   # distinct live buffers
     call('pbsed_event_frames', ptr(x), ptr(th_dev), ptr(ln_dev), ptr(ev), ptr(cnt), r, t, max_events, stream())
     return ev, cnt
+
+
+# ------------------------------------------------------------------------------------- state-space sequence layers
+# Time-major [T, B, channels] like the GRU scans' buffers, in float32, bfloat16 or float16 (parameters, states of the scan and
+# parameter gradients: float32).  Inputs may be slices of wider buffers (unit stride over channels, any over frames and clips);
+# outputs are new contiguous tensors.  ``seq_len`` (int32 [B] or None = T): frames behind it are not read and their outputs are 0;
+# ``reverse``: a clip's valid frames from the last to the first.  Parameter gradients are ADDED to the float32 buffers handed in, in
+# a fixed order.  Launches run on the current stream of the tensors' device; workspaces are allocated per call.
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PBSED_F32 / PBSED_BF16 / PBSED_F16
+
+
+_RAW_STREAM = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, '_cuda_getCurrentRawStream') else None
+
+
+def _fail(name, message):
+    raise ValueError(f'{name}: {message}')
+
+
+def _elem(name, x, dim):
+    """Element-type code and device of the operator's leading tensor [..., channels] with ``dim`` axes (0: any)."""
+    _lib.require_gpu(x)
+    code = DTYPE_CODES.get(x.dtype)
+    if code is None:
+        _fail(name, f'element type {x.dtype}; float32, bfloat16 or float16')
+    if (dim and x.dim() != dim) or not x.dim() or not x.numel():
+        _fail(name, f'expected a {dim or "1 or more"}-d tensor that is not empty, got {tuple(x.shape)}')
+    return code, x.get_device()
+
+
+def _like(name, what, v, shape, dtype, dev, whole=False):
+    """Checks an operand: shape, type, device; unit stride over its channels (``whole``: contiguous).  Returns its address (None: NULL)."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor) or v.shape != shape or v.dtype != dtype or v.get_device() != dev:
+        _fail(name, f'{what} must be a {dtype} tensor of shape {tuple(shape)} on device {dev}, got '
+                    + (f'{v.dtype} {tuple(v.shape)} on {v.device}' if isinstance(v, torch.Tensor) else repr(type(v))))
+    if whole:
+        if not v.is_contiguous():
+            _fail(name, f'{what} must be contiguous')
+    elif shape[-1] != 1 and v.stride(-1) != 1:
+        _fail(name, f'{what} needs unit stride over its channels')
+    return v.data_ptr()
+
+
+def _have(name, what, v, *args):
+    if v is None:
+        _fail(name, f'{what} is missing')
+    return _like(name, what, v, *args)
+
+
+def _launch(dev, entry, *args):
+    """Calls an entry point on the current stream of device ``dev`` (its last argument)."""
+    if dev < 0 or _RAW_STREAM is None:
+        call(entry, *args, stream())
+    elif dev == torch.cuda.current_device():
+        call(entry, *args, _RAW_STREAM(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(entry, *args, _RAW_STREAM(dev))
+
+
+def _on_device(dev, fn, *args):
+    """A size query whose answer depends on the device."""
+    if dev < 0 or dev == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _strides(*tensors):
+    """(frame stride, clip stride) of every [T, B, channels] tensor (None: zeros), as the host array of the C-ABI."""
+    vals = []
+    for t in tensors:
+        vals += (0, 0) if t is None else t.stride()[:2]
+    return (C.c_longlong * len(vals))(*vals)
+
+
+def _span(t):
+    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _distinct(name, what, out, **inputs):
+    """An output handed in by the caller must not share memory with what the launch still reads, nor with itself."""
+    if out is None:
+        return
+    dims = sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1)
+    reach = 1
+    for s, n in dims:
+        if s < reach:
+            _fail(name, f'{what} of strides {out.stride()} overlaps itself')
+        reach = s * (n - 1) + reach
+    lo, hi = out.data_ptr(), out.data_ptr() + _span(out)
+    for key, v in inputs.items():
+        if v is not None and v.data_ptr() < hi and lo < v.data_ptr() + _span(v) and not _interleaved(out, v):
+            _fail(name, f'{what} overlaps {key}')
+
+
+def _interleaved(a, b):
+    """Disjoint channel ranges of one wider buffer: equal strides in front of the channels, multiples of the smallest of them, and the
+    offset between the two modulo that leaves room for both rows."""
+    if a.dim() < 2 or a.shape[:-1] != b.shape[:-1] or a.stride()[:-1] != b.stride()[:-1] or a.element_size() != b.element_size():
+        return False
+    steps = [s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1]
+    pitch = min(steps, default=0)
+    off = b.data_ptr() - a.data_ptr()
+    if pitch <= 0 or off % a.element_size() or any(s % pitch for s in steps):
+        return False
+    off = off // a.element_size() % pitch
+    return off >= a.shape[-1] and off + b.shape[-1] <= pitch
+
+
+def _conv_weight(name, weight, d, dev):
+    if weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
+        _fail(name, f'weight must be [D, K] with 2 <= K <= 8, got {tuple(weight.shape)}')
+    return _have(name, 'weight', weight, (d, weight.shape[1]), torch.float32, dev, True), weight.shape[1]
+
+
+def causal_conv_fwd(x, weight, bias=None, *, silu=True, seq_len=None, reverse=False, state=None, want_state=False):
+    """Causal convolution per channel: x [T,B,D], weight float32 [D,K] (2 <= K <= 8; the last tap meets the current frame), bias [D] or
+    None -> (y [T,B,D], state_out | None).  ``state`` [B,K-1,D] (type of x, oldest first): the positions in front of the first frame,
+    zeros if None; ``state_out``: the last K-1 positions, to hand to the next piece of a recording or to ``causal_conv_step``."""
+    name = 'causal_conv_fwd'
+    code, dev = _elem(name, x, 3)
+    t, b, d = shape = x.shape
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    pw, k = _conv_weight(name, weight, d, dev)
+    pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
+    pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
+    ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
+    y = x.new_empty(shape)
+    state_out = x.new_empty((b, k - 1, d)) if want_state else None
+    st, sb, _ = x.stride()
+    _launch(dev, 'pbsed_causal_conv_fwd', px, pw, pb, pl, ps, y.data_ptr(), state_out.data_ptr() if want_state else None, t, b, d, k, st, sb,
+            int(silu), int(reverse), code)
+    return y, state_out
+
+
+def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=True, seq_len=None, reverse=False, state=None,
+                    dstate_out=None, want_dstate=False, dx=None):
+    """Gradients of ``causal_conv_fwd``: returns (dx [T,B,D], dstate | None); ``dweight`` [D,K] / ``dbias`` [D] (+=).  ``dx``: where to
+    write it (e.g. a channel slice of the projection's gradient) instead of a new tensor; ``dstate_out``: gradient of state_out."""
+    name = 'causal_conv_bwd'
+    code, dev = _elem(name, x, 3)
+    t, b, d = shape = x.shape
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    pg = _have(name, 'dy', dy, shape, x.dtype, dev)
+    pw, k = _conv_weight(name, weight, d, dev)
+    pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
+    pdw = _like(name, 'dweight', dweight, (d, k), torch.float32, dev, True)
+    pdb = _like(name, 'dbias', dbias, (d,), torch.float32, dev, True)
+    pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
+    ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
+    pso = _like(name, 'dstate_out', dstate_out, (b, k - 1, d), x.dtype, dev, True)
+    if dx is None:
+        dx = x.new_empty(shape)
+    else:
+        _like(name, 'dx', dx, shape, x.dtype, dev)
+        _distinct(name, 'dx', dx, x=x, dy=dy, state=state, dstate_out=dstate_out)
+    dstate = x.new_empty((b, k - 1, d)) if want_dstate else None
+    floats = _on_device(dev, _lib.lib().pbsed_causal_conv_workspace, t, b, d, k) if pdw or pdb else 0
+    ws = x.new_empty(floats, dtype=torch.float32) if floats else None
+    gt, gb, _ = dy.stride()
+    xt, xb, _ = x.stride()
+    ot, ob, _ = dx.stride()
+    _launch(dev, 'pbsed_causal_conv_bwd', pg, px, pw, pb, pl, ps, pso, dx.data_ptr(), dstate.data_ptr() if want_dstate else None, pdw, pdb,
+            ws.data_ptr() if floats else None, floats, t, b, d, k, gt, gb, xt, xb, ot, ob, int(silu), int(reverse), code)
+    return dx, dstate
+
+
+def _step_state(name, state, state_out, ps, shape, dtype, dev, **inputs):
+    """Address of where a one-frame form leaves its state: in place, or a buffer that does not overlap what it reads."""
+    if state_out is None or state_out is state:
+        return ps
+    po = _like(name, 'state_out', state_out, shape, dtype, dev, True)
+    if po != ps:
+        lo, hi = po, po + _span(state_out)
+        if ps < hi and lo < ps + _span(state):
+            _fail(name, 'state_out overlaps state')
+    return po
+
+
+def causal_conv_step(x, weight, bias, state, *, silu=True, state_out=None):
+    """One frame of every stream: x [B,D], state [B,K-1,D] -> y [B,D].  The state moves on in place, or into ``state_out``."""
+    name = 'causal_conv_step'
+    code, dev = _elem(name, x, 2)
+    b, d = shape = x.shape
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    pw, k = _conv_weight(name, weight, d, dev)
+    pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
+    ps = _have(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
+    po = _step_state(name, state, state_out, ps, (b, k - 1, d), x.dtype, dev)
+    y = x.new_empty(shape)
+    _launch(dev, 'pbsed_causal_conv_step', px, pw, pb, ps, po, y.data_ptr(), b, d, k, x.stride(0), int(silu), code)
+    return y
+
+
+def _scan_operands(name, dim, u, delta, a_log, b, c, d, z, delta_bias):
+    """Checks what the scan's three forms share: (element code, device, N, addresses of the operands)."""
+    code, dev = _elem(name, u, dim)
+    shape, dt, f32 = u.shape, u.dtype, torch.float32
+    if a_log.dim() != 2 or not 1 <= a_log.shape[1] <= 64:
+        _fail(name, f'a_log must be [D, N] with 1 <= N <= 64, got {tuple(a_log.shape)}')
+    width, n = shape[-1], a_log.shape[1]
+    states = (*shape[:-1], n)
+    return code, dev, n, (_like(name, 'u', u, shape, dt, dev), _have(name, 'delta', delta, shape, dt, dev),
+                          _have(name, 'a_log', a_log, (width, n), f32, dev, True), _have(name, 'b', b, states, dt, dev),
+                          _have(name, 'c', c, states, dt, dev), _like(name, 'd', d, (width,), f32, dev, True),
+                          _like(name, 'z', z, shape, dt, dev), _like(name, 'delta_bias', delta_bias, (width,), f32, dev, True))
+
+
+_SCAN_PLANS = {}        # (device, T, B, D, N, backward) -> (floats of the saved states, of the workspace)
+
+
+def _scan_plan(dev, t, b, d, n, backward):
+    key = (dev, t, b, d, n, backward)
+    plan = _SCAN_PLANS.get(key)
+    if plan is None:
+        saved, ws = C.c_longlong(), C.c_longlong()
+        _on_device(dev, call, 'pbsed_selective_scan_plan', t, b, d, n, int(backward), C.byref(saved), C.byref(ws))
+        if len(_SCAN_PLANS) > 4096:
+            _SCAN_PLANS.clear()
+        plan = _SCAN_PLANS[key] = saved.value, ws.value
+    return plan
+
+
+def selective_scan_fwd(u, delta, a_log, b, c, *, d=None, z=None, delta_bias=None, softplus=True, seq_len=None, reverse=False, state=None,
+                       want_state=False, save=False):
+    """Selective state-space scan: per channel and state  h_t = exp(D_t A) h_{t-1} + D_t u_t b_t,  y_t = (c_t . h_t + d u_t) silu(z_t),
+    D_t = softplus(delta_t + delta_bias) (``softplus=False``: the sum itself), A = -exp(a_log).  u, delta, z [T,B,D]; b, c [T,B,N]; a_log
+    float32 [D,N], N <= 64; d, delta_bias [D]; z / d / delta_bias may be None.  ``state`` float32 [B,D,N]: h in front of the first frame.
+    Returns (y [T,B,D], state_out [B,D,N] | None, saved | None): ``saved`` (``save=True``) is what ``selective_scan_bwd`` takes."""
+    name = 'selective_scan_fwd'
+    code, dev, n, ptrs = _scan_operands(name, 3, u, delta, a_log, b, c, d, z, delta_bias)
+    t, bs, width = u.shape
+    pl = _like(name, 'seq_len', seq_len, (bs,), torch.int32, dev, True)
+    ps = _like(name, 'state', state, (bs, width, n), torch.float32, dev, True)
+    n_saved, n_ws = _scan_plan(dev, t, bs, width, n, False)
+    y = u.new_empty((t, bs, width))
+    state_out = u.new_empty((bs, width, n), dtype=torch.float32) if want_state else None
+    saved = u.new_empty(n_saved, dtype=torch.float32) if save else None
+    ws = u.new_empty(n_ws, dtype=torch.float32) if n_ws else None
+    _launch(dev, 'pbsed_selective_scan_fwd', *ptrs, pl, ps, y.data_ptr(), state_out.data_ptr() if want_state else None,
+            saved.data_ptr() if save else None, ws.data_ptr() if n_ws else None, n_ws, _strides(u, delta, b, c, z), t, bs, width, n,
+            int(softplus), int(reverse), code)
+    return y, state_out, saved
+
+
+def selective_scan_bwd(dy, u, delta, a_log, b, c, saved, *, d=None, z=None, delta_bias=None, softplus=True, seq_len=None, reverse=False,
+                       dstate_out=None, want_dstate=False, da_log=None, dd=None, ddelta_bias=None, dz=None):
+    """Gradients of ``selective_scan_fwd`` (same operands; ``saved``: its third result): returns (du, ddelta [T,B,D], db, dc [T,B,N],
+    dz | None, dstate [B,D,N] | None); ``da_log`` [D,N] / ``dd`` [D] / ``ddelta_bias`` [D] (+=).  ``dstate_out``: gradient of state_out;
+    ``dstate`` (``want_dstate=True``): of state.  ``dz``: where to write it instead of a new tensor."""
+    name = 'selective_scan_bwd'
+    code, dev, n, ptrs = _scan_operands(name, 3, u, delta, a_log, b, c, d, z, delta_bias)
+    t, bs, width = shape = u.shape
+    f32 = torch.float32
+    pg = _have(name, 'dy', dy, shape, u.dtype, dev)
+    pl = _like(name, 'seq_len', seq_len, (bs,), torch.int32, dev, True)
+    pso = _like(name, 'dstate_out', dstate_out, (bs, width, n), f32, dev, True)
+    pda = _like(name, 'da_log', da_log, (width, n), f32, dev, True)
+    pdd = _like(name, 'dd', dd, (width,), f32, dev, True)
+    pdb = _like(name, 'ddelta_bias', ddelta_bias, (width,), f32, dev, True)
+    n_saved, n_ws = _scan_plan(dev, t, bs, width, n, True)
+    psv = _have(name, 'saved', saved, (n_saved,), f32, dev, True)
+    if dz is not None:
+        if z is None:
+            _fail(name, 'dz without z')
+        _like(name, 'dz', dz, shape, u.dtype, dev)
+        _distinct(name, 'dz', dz, dy=dy, u=u, delta=delta, z=z, b=b, c=c)
+    elif z is not None:
+        dz = u.new_empty(shape)
+    du, ddelta = u.new_empty(shape), u.new_empty(shape)
+    db, dc = u.new_empty((t, bs, n)), u.new_empty((t, bs, n))
+    dstate = u.new_empty((bs, width, n), dtype=f32) if want_dstate else None
+    ws = u.new_empty(n_ws, dtype=f32)
+    _launch(dev, 'pbsed_selective_scan_bwd', pg, *ptrs, pl, psv, pso, du.data_ptr(), ddelta.data_ptr(), db.data_ptr(), dc.data_ptr(),
+            None if dz is None else dz.data_ptr(), dstate.data_ptr() if want_dstate else None, pda, pdd, pdb, ws.data_ptr(), n_ws,
+            _strides(u, delta, b, c, z, dy, dz), t, bs, width, n, int(softplus), int(reverse), code)
+    return du, ddelta, db, dc, dz, dstate
+
+
+def selective_scan_step(u, delta, a_log, b, c, state, *, d=None, z=None, delta_bias=None, softplus=True, state_out=None):
+    """One frame of every stream: u, delta, z [B,D]; b, c [B,N]; state float32 [B,D,N] -> y [B,D].  The state moves on in place, or
+    into ``state_out``."""
+    name = 'selective_scan_step'
+    code, dev, n, ptrs = _scan_operands(name, 2, u, delta, a_log, b, c, d, z, delta_bias)
+    bs, width = u.shape
+    ps = _have(name, 'state', state, (bs, width, n), torch.float32, dev, True)
+    po = _step_state(name, state, state_out, ps, (bs, width, n), torch.float32, dev)
+    y = u.new_empty((bs, width))
+    strides = (C.c_longlong * 5)(u.stride(0), delta.stride(0), b.stride(0), c.stride(0), 0 if z is None else z.stride(0))
+    _launch(dev, 'pbsed_selective_scan_step', *ptrs, ps, po, y.data_ptr(), strides, bs, width, n, int(softplus), code)
+    return y
+
+
+def _row_stride(name, what, v):
+    """The one stride between the rows of a [..., C] tensor."""
+    shape, strides = v.shape, v.stride()
+    c = shape[-1]
+    row, rows = None, 1                                     # from the innermost axis outwards: every axis continues the one inside it
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if row is None:
+            row = s
+        elif s != row * rows:
+            _fail(name, f'{what} of shape {tuple(shape)} and strides {tuple(strides)} has no single row stride')
+        rows *= n
+    row = c if row is None else row
+    if row < c:
+        _fail(name, f'{what} of strides {tuple(strides)} has overlapping rows')
+    return row
+
+
+def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5, save=False):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., C]; weight, bias float32 [C] or None.  Returns (y, stats |
+    None): ``stats`` (``save=True``) is what ``layer_norm_bwd`` takes."""
+    name = 'layer_norm_fwd'
+    code, dev = _elem(name, x, 0)
+    shape = x.shape
+    c = shape[-1]
+    rows = x.numel() // c
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    xs = _row_stride(name, 'x', x)
+    pw = _like(name, 'weight', weight, (c,), torch.float32, dev, True)
+    pb = _like(name, 'bias', bias, (c,), torch.float32, dev, True)
+    if not eps >= 0:
+        _fail(name, f'eps = {eps}')
+    y = x.new_empty(shape)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if save else None
+    _launch(dev, 'pbsed_layer_norm_fwd', px, pw, pb, y.data_ptr(), stats.data_ptr() if save else None, rows, c, xs, float(eps), code)
+    return y, stats
+
+
+def layer_norm_bwd(dy, x, weight, stats, *, dweight=None, dbias=None):
+    """Gradients of ``layer_norm_fwd``: returns dx; ``dweight`` / ``dbias`` [C] (+=)."""
+    name = 'layer_norm_bwd'
+    code, dev = _elem(name, x, 0)
+    shape = x.shape
+    c = shape[-1]
+    rows = x.numel() // c
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    pg = _have(name, 'dy', dy, shape, x.dtype, dev)
+    pw = _like(name, 'weight', weight, (c,), torch.float32, dev, True)
+    pst = _have(name, 'stats', stats, (rows, 2), torch.float32, dev, True)
+    pdw = _like(name, 'dweight', dweight, (c,), torch.float32, dev, True)
+    pdb = _like(name, 'dbias', dbias, (c,), torch.float32, dev, True)
+    dx = x.new_empty(shape)
+    floats = _on_device(dev, _lib.lib().pbsed_layer_norm_workspace, rows, c) if pdw or pdb else 0
+    ws = x.new_empty(floats, dtype=torch.float32) if floats else None
+    _launch(dev, 'pbsed_layer_norm_bwd', pg, px, pw, pst, dx.data_ptr(), pdw, pdb, ws.data_ptr() if floats else None, floats, rows, c,
+            _row_stride(name, 'dy', dy), _row_stride(name, 'x', x), code)
+    return dx
+
+
+def dropout(x, p, rng, *, site=0, residual=None, out=None):
+    """[residual +] x / (1 - p) where element i (row-major) of the mask is kept, else [residual +] 0.  The mask is a function of ``rng``
+    (int64 [2] on the device: seed, step), ``site`` (which dropout of the step, 0 <= site < 2^31) and i, never stored: the backward pass
+    is ``dropout(dy, p, rng, site=site)`` with the same three.  Advance ``rng[1]`` (modulo 2^32) for a new mask, also between the replays
+    of a captured graph.  ``out``: where to write (may be x or residual)."""
+    name = 'dropout'
+    code, dev = _elem(name, x, 0)
+    shape = x.shape
+    c = shape[-1]
+    if not 0. <= p <= 1.:
+        _fail(name, f'p = {p} is not in [0, 1]')
+    if not 0 <= site < 1 << 31:
+        _fail(name, f'site = {site}')
+    px = _like(name, 'x', x, shape, x.dtype, dev)
+    pr = _have(name, 'rng', rng, (2,), torch.int64, dev, True)
+    pres = _like(name, 'residual', residual, shape, x.dtype, dev)
+    if out is None:
+        out = x.new_empty(shape)
+    else:
+        _like(name, 'out', out, shape, x.dtype, dev)
+        same = {key: v for key, v in (('x', x), ('residual', residual))
+                if v is not None and not (v.data_ptr() == out.data_ptr() and v.stride() == out.stride())}
+        _distinct(name, 'out', out, rng=rng, **same)
+    _launch(dev, 'pbsed_dropout', px, pres, out.data_ptr(), x.numel() // c, c, _row_stride(name, 'x', x),
+            0 if residual is None else _row_stride(name, 'residual', residual), _row_stride(name, 'out', out), code, float(p), pr, int(site))
+    return out

@@ -24,7 +24,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 CLANG = '/opt/rocm/lib/llvm/bin/clang++'
 OPT = os.environ.get('PBSED_EMU_OPT', '-O0').split()
-UNITS = ('api', 'conv_s16', 'conv_winox3', 'conv_wino', 'conv_bf16', 'conv1d_pc', 'logmel', 'gru', 'gru_stack', 'rnn_gemms', 'postproc')
+UNITS = ('api', 'conv_s16', 'conv_winox3', 'conv_wino', 'conv_bf16', 'conv1d_pc', 'logmel', 'gru', 'gru_stack', 'rnn_gemms', 'postproc', 'sequence')
 
 
 def compile_unit(unit, csrc, out, defines=()):

@@ -186,6 +186,7 @@ static inline int __builtin_amdgcn_update_dpp(int old, int src, int ctrl, int ro
     if (ctrl < 0x100) from = (l & ~3) + ((ctrl >> (2 * (l & 3))) & 3);                  // quad_perm
     else if (ctrl >= 0x101 && ctrl <= 0x10F) from = p + (ctrl - 0x100) <= 15 ? l + (ctrl - 0x100) : -1;     // row_shl:n reads lane + n
     else if (ctrl >= 0x111 && ctrl <= 0x11F) from = p - (ctrl - 0x110) >= 0 ? l - (ctrl - 0x110) : -1;      // row_shr:n reads lane - n
+    else if (ctrl >= 0x121 && ctrl <= 0x12F) from = row + ((p - (ctrl - 0x120)) & 15);   // row_ror:n reads lane - n, round the row
     else if (ctrl == 0x140) from = row + 15 - p;                                         // row_mirror
     else if (ctrl == 0x141) from = row + (p & 8) + 7 - (p & 7);                          // row_half_mirror
     else { fprintf(stderr, "hipemu: dpp control 0x%x not emulated\n", ctrl); abort(); }
@@ -194,6 +195,22 @@ static inline int __builtin_amdgcn_update_dpp(int old, int src, int ctrl, int ro
     hipemu::wave_sync();
     return r;
 }
+// v_permlane32_swap / v_permlane16_swap: the upper half (the odd 16-lane rows) of x change places with the lower half (the even rows) of y
+typedef unsigned hipemu_swap2 __attribute__((ext_vector_type(2)));
+static inline hipemu_swap2 hipemu_swap(unsigned x, unsigned y, int span) {
+    hipemu::Wave& w = hipemu::my_wave();
+    const int l = hipemu::lane();
+    const unsigned v[2] = {x, y};
+    memcpy(w.slot[l], v, 8);
+    hipemu::wave_sync();
+    unsigned o[2] = {x, y};
+    if (l & span) memcpy(&o[0], w.slot[l - span] + 4, 4);
+    else memcpy(&o[1], w.slot[l + span], 4);
+    hipemu::wave_sync();
+    return hipemu_swap2{o[0], o[1]};
+}
+static inline hipemu_swap2 __builtin_amdgcn_permlane32_swap(unsigned x, unsigned y, bool, bool) { return hipemu_swap(x, y, 32); }
+static inline hipemu_swap2 __builtin_amdgcn_permlane16_swap(unsigned x, unsigned y, bool, bool) { return hipemu_swap(x, y, 16); }
 static inline unsigned __builtin_amdgcn_perm(unsigned a, unsigned b, unsigned sel) {       // v_perm_b32: bytes 0..3 of b, 4..7 of a
     const unsigned char src[8] = {(unsigned char)b, (unsigned char)(b >> 8), (unsigned char)(b >> 16), (unsigned char)(b >> 24),
                                   (unsigned char)a, (unsigned char)(a >> 8), (unsigned char)(a >> 16), (unsigned char)(a >> 24)};

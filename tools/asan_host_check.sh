@@ -15,7 +15,7 @@ mkdir -p $W/build
 cd $ROOT/pb_sed_amd/csrc
 FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC $SAN -fno-gpu-sanitize -fno-omit-frame-pointer -Wno-unused-result -Wno-unused-value"
 pids=()
-for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm misc logmel postproc collective; do
+for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm causal_conv selective_scan layer_norm dropout misc logmel postproc collective; do
   /opt/rocm/bin/hipcc $FLAGS -c $f.hip -o $W/build/$f.o 2> $W/build/$f.err &
   pids+=($!)
 done
