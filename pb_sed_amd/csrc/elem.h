@@ -33,18 +33,15 @@ __device__ __forceinline__ float exp_neg(float x) {
     const float e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, l * 0.69314718f, e);
 }
-// log(1 + exp(x)) without cancellation: max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], and log1p(e) = 2 atanh(s) with
-// s = e / (2 + e) <= 1/3 as its Taylor series in s^2 <= 1/9 (the first term left out is 9^-8 / 17 of the sum: below 2^-29)
+// log(1 + exp(x)) without cancellation: max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], and log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
+// with atanh(s) / s as the polynomial of degree four in s^2 that meets it at the Chebyshev nodes of [0, 1/9] (relative error 8e-9)
 __device__ __forceinline__ float softplus(float x) {
     const float e = exp_neg(fminf(fabsf(x), 100.f));
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float p = 1.f / 15.f;
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
+    float p = 0.14078889788f;
+    p = fmaf(p, q, 0.13982579112f);
+    p = fmaf(p, q, 0.20012298226f);
+    p = fmaf(p, q, 0.33333161473f);
     p = fmaf(p, q, 1.f);
     const float y = fmaf(2.f * s, p, fmaxf(x, 0.f));
     return x != x ? x : y;                                          // v_max_f32 would drop a NaN

@@ -8,16 +8,15 @@
 //     ddelta = dD sigmoid(raw),   da_log = A sum_{t,b} r D q,   dskip = sum g u,   dz = dy (C.h + skip u) silu'(z)
 // Frames behind a clip's end are not read, their outputs are 0, and the state stands still.
 //
-// Layout: LN lanes share a channel, four states each (LN = 1, 2, 4, 8, 16 for up to 4 ... 64 states), so a wave holds 64 / LN channels
-// and its states never leave registers; y is a sum of four terms per lane and log2(LN) DPP adds.  A block of four waves stages a tile
-// of frames: softplus, the products with u and the gate are computed once per element, coalesced along the channels, and handed to
-// the lanes through LDS transposed (four consecutive frames of a channel are one 16-byte read).
-// The decay over a run of frames is exp(A sum D): a run's effect on the state is (sum D, its end state from zero).  Where B and the
-// channels alone do not fill the device, the frames are cut into runs: a first launch leaves every run's (sum D, end state), the main
-// launch folds the runs in front of its own into its initial state (backward: the runs behind it into its adjoint).
-//
-// Bound: forward by the exponentials - B T D N of them at a quarter of the VALU rate beside five ordinary instructions each -, about
-// level with HBM for N = 16 in float.
+// Layout: LN lanes share a channel, NS states each (N <= 8: 4 x 2, <= 16: 8 x 2, <= 32: 16 x 2, <= 64: 16 x 4), so a wave holds
+// 64 / LN channels and its states never leave registers; y is a sum of NS terms per lane and log2(LN) DPP adds.  A block of four waves
+// stages a tile of frames: softplus, the products with u and the gate are computed once per element, coalesced along the channels, and
+// handed to the lanes through LDS transposed (four consecutive frames of a channel are one 16-byte read).
+// The decay over a run of frames is exp(A sum D): a run's effect on the state is (sum D, its end state from zero).  Where clips and
+// channels alone do not fill the device, the frames are cut into runs: a first launch leaves every run's (sum D, end state), and the
+// main launch starts from the state in front of its run (backward: from the adjoint behind it).
+#include <type_traits>
+
 #include "elem.h"
 #include "pbsed_internal.h"
 
@@ -36,26 +35,30 @@ struct ScanArgs {
     float* sums;                                       // backward: [B nrun][D N + 2 D] partial sums of da_log | dskip | ddelta_bias
     long long ut, ub, et, eb, bt, bb, ct, cb, zt, zb, gt, gb, dzt, dzb;      // strides over frames and clips (elements)
     int T, B, D, N, reverse, softplus, nrun, run;      // run: frames per run, a multiple of 64
+    int folded;                                        // runs hold the states in front of the runs (scan_runs_kernel has been there)
 };
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr int SC_SAVE = 16;                            // frames between saved states; also the tile of the backward kernel
 
+template <int CTRL> __device__ __forceinline__ float dpp_lane(float v) {        // every lane has a source: folds into the addition
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int LN> __device__ __forceinline__ float lanes_sum(float v) {          // over the LN lanes of a channel
-    if constexpr (LN >= 2) v += dpp_shuffled<0xB1>(v);       // quad_perm [1,0,3,2]
-    if constexpr (LN >= 4) v += dpp_shuffled<0x4E>(v);       // quad_perm [2,3,0,1]
-    if constexpr (LN >= 8) v += dpp_shuffled<0x141>(v);      // row_half_mirror
-    if constexpr (LN >= 16) v += dpp_shuffled<0x140>(v);     // row_mirror
+    if constexpr (LN >= 2) v += dpp_lane<0xB1>(v);       // quad_perm [1,0,3,2]
+    if constexpr (LN >= 4) v += dpp_lane<0x4E>(v);       // quad_perm [2,3,0,1]
+    if constexpr (LN >= 8) v += dpp_lane<0x141>(v);      // row_half_mirror
+    if constexpr (LN >= 16) v += dpp_lane<0x140>(v);     // row_mirror
     return v;
 }
-// the four states n0 .. n0+3 of a row of N floats (zeros behind N)
-__device__ __forceinline__ void load_states(const float* row, int n0, int N, float (&v)[4]) {
+// the NS states from n0 on of a row of N floats (zeros behind N)
+template <int NS> __device__ __forceinline__ void load_states(const float* row, int n0, int N, float (&v)[NS]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = n0 + j < N ? row[n0 + j] : 0.f;
+    for (int j = 0; j < NS; ++j) v[j] = n0 + j < N ? row[n0 + j] : 0.f;
 }
-__device__ __forceinline__ void store_states(float* row, int n0, int N, const float (&v)[4]) {
+template <int NS> __device__ __forceinline__ void store_states(float* row, int n0, int N, const float (&v)[NS]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < NS; ++j)
         if (n0 + j < N) row[n0 + j] = v[j];
 }
 __device__ __forceinline__ float4 f4(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
@@ -66,236 +69,396 @@ __device__ __forceinline__ float rate_of(float a_log) {
     return v > 1e37f ? 1e37f : v;
 }
 __device__ __forceinline__ float step_of(const ScanArgs& a, float raw) { return a.softplus ? softplus(raw) : raw; }
-
-// h of a channel's lane in front of run c: h0 and the runs before it
-template <int LN>
-__device__ __forceinline__ void fold_runs(const ScanArgs& a, int from, int to, int dir, int b, int d, int nq, const float (&A2)[4], float (&h)[4]) {
-    constexpr int NP = 4 * LN;
-#pragma unroll 4
-    for (int c = from; c != to; c += dir) {
-        const long long at_ = ((long long)c * a.B + b) * a.D + d;
-        const float4 s = *reinterpret_cast<const float4*>(a.runs + at_ * NP + nq * 4);
-        const float dt = a.runs_dt[at_];
+// D of F frames of a channel, 0 for those that do not exist (frames F sq + i >= left of a tile); the uniform choices stand outside, so that
+// the F chains interleave
+template <int F> __device__ __forceinline__ void steps_of(const ScanArgs& a, const float (&raw)[F], float bias, int first, int left, float (&D)[F]) {
+    if (a.softplus) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], at(s, j));
+        for (int i = 0; i < F; ++i) D[i] = softplus(raw[i] + bias);
+    } else {
+#pragma unroll
+        for (int i = 0; i < F; ++i) D[i] = raw[i] + bias;
+    }
+    if (left < first + F)
+#pragma unroll
+        for (int i = 0; i < F; ++i) D[i] = first + i < left ? D[i] : 0.f;
+}
+
+// h of a channel's lane in front of run c: the start value and the runs from `from` to `to` (outside)
+template <int LN, int NS>
+__device__ __forceinline__ void fold_runs(const ScanArgs& a, int c, int from, int to, int dir, int b, int d, int nq, const float (&A2)[NS], float (&h)[NS]) {
+    constexpr int NP = NS * LN;
+    if (a.folded) {
+        load_pack<float, NS>(a.runs + (((long long)c * a.B + b) * a.D + d) * NP + nq * NS, h);
+        return;
+    }
+#pragma unroll 8
+    for (int k = from; k != to; k += dir) {
+        const long long i = ((long long)k * a.B + b) * a.D + d;
+        float s[NS];
+        load_pack<float, NS>(a.runs + i * NP + nq * NS, s);
+        const float dt = a.runs_dt[i];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], s[j]);
+    }
+}
+// Many runs (up to 256): their end states become the states in front of them, in place.  A lane owns one state; wave w of a block's 16
+// takes runs 16 w .. 16 w + 15 of the order, holds them in registers, and learns through LDS what the waves in front of it add up to.
+// back: from the last run to the first, starting from dh_out.
+__global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int back) {
+    __shared__ float ss[16][64], sp[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long M = (long long)a.B * a.D * NP, m = (long long)blockIdx.x * 64 + lane;
+    const bool on = m < M;
+    const long long bd = on ? m / NP : 0;
+    const int n = (int)(m % NP), d = (int)(bd % a.D);
+    const float A2 = on && n < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : 0.f;
+    const float* start = back ? a.dh_out : a.h0;
+    const float x0 = start && on && n < a.N ? start[bd * a.N + n] : 0.f;
+    float s[16], dt[16], S = 0.f, P = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int k = wave * 16 + i, c = back ? a.nrun - 1 - k : k;
+        const bool has = on && k < a.nrun - 1;                       // (nothing lies behind the last one: it left no end state)
+        s[i] = has ? a.runs[(long long)c * M + m] : 0.f;
+        dt[i] = has ? a.runs_dt[(long long)c * (M / NP) + bd] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        S = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2), S, s[i]);
+        P += dt[i];
+    }
+    ss[wave][lane] = S;
+    sp[wave][lane] = P;
+    __syncthreads();
+    float x = x0;
+    for (int w = 0; w < wave; ++w) x = fmaf(__builtin_amdgcn_exp2f(sp[w][lane] * A2), x, ss[w][lane]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int k = wave * 16 + i, c = back ? a.nrun - 1 - k : k;
+        if (on && k < a.nrun) a.runs[(long long)c * M + m] = x;
+        x = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2), x, s[i]);
     }
 }
 
+// Tiles are loaded through buffer resources based at the tile's first frame in memory: a lane's offset inside the tile is a constant, the
+// rows of its four frames differ by a scalar offset, and elements that do not exist (frames behind the clip's end, channels behind D)
+// get an offset out of range - they read 0 and are not stored, without a branch whose two sides the wait counters would have to cover.
+constexpr unsigned SC_OUT = 0x80000000u;
+template <class S> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const S* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(p), 0, 0x7fffffffu, 0x00020000);
+}
+template <class S> __device__ __forceinline__ float row_load(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff) {
+    if constexpr (sizeof(S) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0));
+    else return (float)__builtin_bit_cast(S, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, 0));
+}
+template <class S> __device__ __forceinline__ void row_store(float v, __amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff) {
+    if constexpr (sizeof(S) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, voff, soff, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (S)v), r, voff, soff, 0);
+}
+// Everything of a wave's earlier loads into v has arrived: inside a loop the compiler would otherwise wait for them - and with them for
+// the loads that are meant to stay under way - at the first use in every turn.
+template <int NS> __device__ __forceinline__ void arrived(float (&v)[NS]) {        // (also: v is computed here, not inside a later branch)
+#ifndef HIP_EMU
+#pragma unroll
+    for (int j = 0; j < NS; ++j) asm volatile("" : "+v"(v[j]));
+#endif
+}
+// offsets of a lane's F frames (F sq .. F sq + F-1 of a tile of TT) in column `col`, out of range where the lane has none
+template <class S, int F> struct LaneRows {
+    unsigned v[F];
+    __device__ __forceinline__ LaneRows(long long stride, int TT, int sq, int col, int reverse, bool on) {
+        const unsigned st = (unsigned)(stride * (long long)sizeof(S));
+#pragma unroll
+        for (int i = 0; i < F; ++i) v[i] = on ? (unsigned)(reverse ? TT - 1 - (F * sq + i) : F * sq + i) * st + (unsigned)(col * (int)sizeof(S)) : SC_OUT;
+    }
+    // the frames of a full tile, or of a tile whose frames from `left` on do not exist
+    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int sq, int left, float (&x)[F]) const {
+#pragma unroll
+        for (int i = 0; i < F; ++i) x[i] = row_load<S>(r, FULL || F * sq + i < left ? v[i] : SC_OUT, 0);
+    }
+    template <bool FULL> __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, int sq, int left, const float (&x)[F]) const {
+#pragma unroll
+        for (int i = 0; i < F; ++i) row_store<S>(x[i], r, FULL || F * sq + i < left ? v[i] : SC_OUT, 0);
+    }
+};
+// the same for a tile of the states' inputs B or C [TT][NP]: element tid + 256 k
+template <class S, int TT, int NP> struct StateRows {
+    static constexpr int NB = TT * NP / 256 > 0 ? TT * NP / 256 : 1;
+    unsigned v[NB];
+    __device__ __forceinline__ StateRows(long long stride, int N, int reverse) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const int i = threadIdx.x + 256 * k, m = i / NP, n = i % NP;
+            v[k] = i < TT * NP && n < N ? ((unsigned)(reverse ? TT - 1 - m : m) * (unsigned)stride + (unsigned)n) * (unsigned)sizeof(S) : SC_OUT;
+        }
+    }
+    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int left, float (&x)[NB]) const {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) x[k] = row_load<S>(r, FULL || ((int)threadIdx.x + 256 * k) / NP < left ? v[k] : SC_OUT, 0);
+    }
+    __device__ __forceinline__ void put(float* lds, const float (&x)[NB]) const {
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+            if (TT * NP >= 256 || (int)threadIdx.x + 256 * k < TT * NP) lds[threadIdx.x + 256 * k] = x[k];
+    }
+};
+
+// Blocks of consecutive ids run on different XCDs; neighbouring channel blocks whose rows share 128-byte lines are put on one (its L2
+// then reads the line once): groups of G blocks, dealt to the XCDs in turn.
+struct ScanBlock { int x, b, c; };
+template <class S, int CB> __device__ __forceinline__ ScanBlock scan_block() {
+    constexpr unsigned G = 128 / (CB * sizeof(S)) > 1 ? 128 / (CB * sizeof(S)) : 1;
+    if constexpr (G == 1) return ScanBlock{(int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z};
+    const unsigned total = gridDim.x * gridDim.y * gridDim.z, id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    unsigned w = id;
+    if (id < total / (8 * G) * (8 * G)) w = ((id >> 3) / G * 8 + (id & 7)) * G + (id >> 3) % G;
+    return ScanBlock{(int)(w % gridDim.x), (int)(w / gridDim.x % gridDim.y), (int)(w / gridDim.x / gridDim.y)};
+}
+
+// LDS operands of four frames of the compute phase, read one group ahead of their use
+template <int NS, bool C> struct ScanGroup {
+    float4 D, U;
+    Pack<float, NS> B[4], Cv[C ? 4 : 1];
+    template <int NP> __device__ __forceinline__ void load(const float* rowD, const float* rowU, const float* sB, const float* sC, int q, int nq) {
+        D = *reinterpret_cast<const float4*>(rowD + 4 * q);
+        U = *reinterpret_cast<const float4*>(rowU + 4 * q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            B[i] = *reinterpret_cast<const Pack<float, NS>*>(sB + (4 * q + i) * NP + nq * NS);
+            if constexpr (C) Cv[i] = *reinterpret_cast<const Pack<float, NS>*>(sC + (4 * q + i) * NP + nq * NS);
+        }
+    }
+};
+
 // grid (channel blocks, B, runs).  SUMMARY: leave this run's end state from zero and sum of D; otherwise the outputs.
-template <class S, int LN, bool SUMMARY>
+template <class S, int LN, int NS, bool SUMMARY>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
-    constexpr int NP = 4 * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4, NBC = (TT * NP + 255) / 256;
+    constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4;
+    using Rows = LaneRows<S, 4>;
+    using BC = StateRows<S, TT, NP>;
     __shared__ __attribute__((aligned(16))) float sD[2][CB * LD], sU[2][CB * LD], sB[2][TT * NP], sC[2][SUMMARY ? 4 : TT * NP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     const int ch = wave * (64 / LN) + lane / LN;                 // the lane's channel of the block
-    const int b = blockIdx.y, c = blockIdx.z, d = blockIdx.x * CB + ch;
-    const int sch = tid % CB, sq = tid / CB, sd = blockIdx.x * CB + sch;       // staging: channel, group of four frames
-    const bool chan = sd < a.D;
+    const ScanBlock blk = scan_block<S, CB>();
+    const int b = blk.b, c = blk.c, d0 = blk.x * CB, d = d0 + ch;
+    const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;       // staging: channel, group of four frames
+    const bool chan = sd < a.D, gated = a.z != nullptr;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
-    const int p0 = c * a.run, p1 = min(p0 + a.run, a.T);
-    const S* u = static_cast<const S*>(a.u) + b * a.ub + sd;
-    const S* e = static_cast<const S*>(a.delta) + b * a.eb + sd;
-    const S* z = static_cast<const S*>(a.z) + b * a.zb + sd;
-    const S* bm = static_cast<const S*>(a.b) + b * a.bb;
-    const S* cm = static_cast<const S*>(a.c) + b * a.cb;
-    auto frame = [&](int p) { return (long long)(a.reverse && p < len ? len - 1 - p : p); };
+    const int p0 = c * a.run, p1 = min(p0 + a.run, a.T), stop = min(p1, len);      // tiles behind `stop` hold nothing
+    const long long yt = (long long)a.B * a.D;
+    // the tile's first frame in memory; a part-filled tile of a reversed clip starts in front of the clip (its frames there do not exist)
+    const long long f0 = a.reverse ? (long long)len - p0 - TT : p0, adv = a.reverse ? -TT : TT;
+    const S* u = static_cast<const S*>(a.u) + b * a.ub + d0 + f0 * a.ut;
+    const S* e = static_cast<const S*>(a.delta) + b * a.eb + d0 + f0 * a.et;
+    const S* z = static_cast<const S*>(a.z) + b * a.zb + d0 + f0 * a.zt;
+    const S* bm = static_cast<const S*>(a.b) + b * a.bb + f0 * a.bt;
+    const S* cm = static_cast<const S*>(a.c) + b * a.cb + f0 * a.ct;
+    S* y = static_cast<S*>(a.y) + (long long)b * a.D + d0 + f0 * yt;
+    const Rows ou(a.ut, TT, sq, sch, a.reverse, chan), oe(a.et, TT, sq, sch, a.reverse, chan);
+    const Rows oz(a.zt, TT, sq, sch, a.reverse, chan & gated), oy(yt, TT, sq, sch, a.reverse, chan);
+    const BC ob(a.bt, a.N, a.reverse), oc(a.ct, a.N, a.reverse);
     const float bias = chan && a.dbias ? a.dbias[sd] : 0.f, skip = chan && a.skip ? a.skip[sd] : 0.f;
 
-    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
-    if (d < a.D) {
-        load_states(a.a_log + (long long)d * a.N, nq * 4, a.N, A2);
+    float A2[NS], h[NS] = {}, dsum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) A2[j] = -LOG2E * rate_of(A2[j]);
-        if (!SUMMARY) {
-            if (a.h0) load_states(a.h0 + ((long long)b * a.D + d) * a.N, nq * 4, a.N, h);
-            fold_runs<LN>(a, 0, c, 1, b, d, nq, A2, h);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) A2[j] = 0.f;
+    for (int j = 0; j < NS; ++j) A2[j] = d < a.D && nq * NS + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
+    if (!SUMMARY && d < a.D) {
+        if (a.h0) load_states<NS>(a.h0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, h);
+        if (a.nrun > 1) fold_runs<LN, NS>(a, c, 0, c, 1, b, d, nq, A2, h);
     }
+    arrived(h);
 
-    float ru[4], re[4], rz[4], rb[NBC], rc[NBC];                  // the next tile's elements on their way
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            const bool on = chan && p < len;
-            const long long f = frame(p);
-            ru[i] = on ? (float)u[f * a.ut] : 0.f;
-            re[i] = on ? (float)e[f * a.et] : 0.f;
-            rz[i] = !SUMMARY && on && a.z ? (float)z[f * a.zt] : 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k, p = t0 + i / NP, n = i % NP;
-            const bool on = i < TT * NP && p < len && n < a.N;
-            rb[k] = on ? (float)bm[frame(p) * a.bt + n] : 0.f;
-            rc[k] = !SUMMARY && on ? (float)cm[frame(p) * a.ct + n] : 0.f;
+    float ru[4], re[4], rz[4], rb[BC::NB], rc[BC::NB];            // the next tile's elements on their way
+    auto request = [&](auto full, int left) __attribute__((always_inline)) {
+        ou.template load<full()>(rows_at(u), sq, left, ru);
+        oe.template load<full()>(rows_at(e), sq, left, re);
+        ob.template load<full()>(rows_at(bm), left, rb);
+        if (!SUMMARY) {
+            oz.template load<full()>(rows_at(z), sq, left, rz);
+            oc.template load<full()>(rows_at(cm), left, rc);
         }
     };
-    const int stop = min(p1, len);                               // tiles behind it hold nothing
+    auto fetch = [&](int left) __attribute__((always_inline)) {
+        if (left >= TT) request(std::true_type(), left);
+        else request(std::false_type(), left);
+        u += adv * a.ut; e += adv * a.et; z += adv * a.zt; bm += adv * a.bt; cm += adv * a.ct;
+    };
     int t0 = p0, buf = 0;
-    if (t0 < stop) fetch(t0);
+    if (t0 < stop) {
+        fetch(len - t0);
+        // as many stores (dropped: out of range) behind the first loads as every turn leaves behind its own: the wait counters count loads
+        // and stores in one order, and only what is the same on both ways into the loop is not waited for
+        if (!SUMMARY)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row_store<S>(0.f, rows_at(y), SC_OUT, 4 * i);
+    }
     for (; t0 < stop; t0 += TT, buf ^= 1) {
-        float us[4], gate[4], D4[4], U4[4];
+        float uc[4], gate[4], D4[4], U4[4];
+        steps_of<4>(a, re, bias, sq * 4, len - t0, D4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            D4[i] = chan && p < len ? step_of(a, re[i] + bias) : 0.f;
             U4[i] = D4[i] * ru[i];
-            us[i] = ru[i] * skip;
-            gate[i] = a.z ? rz[i] * fast_sigmoid(rz[i]) : 1.f;
+            uc[i] = ru[i];
+            gate[i] = 1.f;
         }
-        *reinterpret_cast<float4*>(&sD[buf][sch * LD + sq * 4]) = f4(D4);
-        *reinterpret_cast<float4*>(&sU[buf][sch * LD + sq * 4]) = f4(U4);
+        if (!SUMMARY && a.z)
 #pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k;
-            if (i < TT * NP) {
-                sB[buf][i] = rb[k];
-                if (!SUMMARY) sC[buf][i] = rc[k];
-            }
-        }
+            for (int i = 0; i < 4; ++i) gate[i] = rz[i] * fast_sigmoid(rz[i]);
+        store_pack<float, 4>(&sD[buf][sch * LD + sq * 4], D4);
+        store_pack<float, 4>(&sU[buf][sch * LD + sq * 4], U4);
+        ob.put(sB[buf], rb);
+        if (!SUMMARY) oc.put(sC[buf], rc);
         __syncthreads();
-        if (t0 + TT < stop) fetch(t0 + TT);
+        if (t0 + TT < stop) fetch(len - t0 - TT);
         float* rowD = &sD[buf][ch * LD];
         const float* rowU = &sU[buf][ch * LD];
+        ScanGroup<NS, !SUMMARY> g;
+        g.template load<NP>(rowD, rowU, sB[buf], sC[buf], 0, nq);
 #pragma unroll
         for (int q = 0; q < TT / 4; ++q) {
-            if (!SUMMARY && a.saved && ((t0 + 4 * q) & (SC_SAVE - 1)) == 0 && d < a.D && t0 + 4 * q < a.T)
-                *reinterpret_cast<float4*>(a.saved + (((long long)((t0 + 4 * q) / SC_SAVE) * a.B + b) * a.D + d) * NP + nq * 4) = f4(h);
-            const float4 dt4 = *reinterpret_cast<const float4*>(rowD + 4 * q), du4 = *reinterpret_cast<const float4*>(rowU + 4 * q);
-            float y4[4];
+            if (!SUMMARY && 4 * q % SC_SAVE == 0 && a.saved && (TT >= SC_SAVE || t0 % SC_SAVE == 0) && d < a.D && (q == 0 || t0 + 4 * q < a.T))
+                store_pack<float, NS>(a.saved + (((long long)((t0 + 4 * q) / SC_SAVE) * a.B + b) * a.D + d) * NP + nq * NS, h);
+            ScanGroup<NS, !SUMMARY> next;
+            if (q + 1 < TT / 4) next.template load<NP>(rowD, rowU, sB[buf], sC[buf], q + 1, nq);
+            __builtin_amdgcn_sched_barrier(0);
+            float ex[4][NS], x[4][NS], y4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    ex[i][j] = __builtin_amdgcn_exp2f(at(g.D, i) * A2[j]);
+                    x[i][j] = at(g.U, i) * g.B[i].v[j];
+                }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float dt = at(dt4, i), du = at(du4, i);
-                const float4 Bv = *reinterpret_cast<const float4*>(&sB[buf][(4 * q + i) * NP + nq * 4]);
-                float4 Cv = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (!SUMMARY) Cv = *reinterpret_cast<const float4*>(&sC[buf][(4 * q + i) * NP + nq * 4]);
-                float y = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], du * at(Bv, j));
-                    if (!SUMMARY) y = fmaf(at(Cv, j), h[j], y);
+                for (int j = 0; j < NS; ++j) {
+                    h[j] = fmaf(ex[i][j], h[j], x[i][j]);
+                    if constexpr (!SUMMARY) y4[i] = j ? fmaf(g.Cv[i].v[j], h[j], y4[i]) : g.Cv[i].v[j] * h[j];
                 }
-                if (SUMMARY) dsum += dt;
-                else y4[i] = lanes_sum<LN>(y);
+                if (SUMMARY) dsum += at(g.D, i);
             }
-            if (!SUMMARY && nq == 0) *reinterpret_cast<float4*>(rowD + 4 * q) = f4(y4);      // the channel's lanes have read D there
+            if constexpr (!SUMMARY) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y4[i] = lanes_sum<LN>(y4[i]);
+                arrived(y4);
+                if (nq == 0) store_pack<float, 4>(rowD + 4 * q, y4);                     // the channel's lanes have read D there
+            }
+            if (q + 1 < TT / 4) g = next;
         }
         if (SUMMARY) continue;
         __syncthreads();
-        const float4 y4 = *reinterpret_cast<const float4*>(&sD[buf][sch * LD + sq * 4]);
-        S* y = static_cast<S*>(a.y) + (long long)b * a.D + sd;
+        float o[4];
+        load_pack<float, 4>(&sD[buf][sch * LD + sq * 4], o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            if (chan && p < p1) y[frame(p) * a.B * a.D] = (S)(p < len ? (at(y4, i) + us[i]) * gate[i] : 0.f);
-        }
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(uc[i], skip, o[i]) * gate[i];
+        if (len - t0 >= TT) oy.template store<true>(rows_at(y), sq, TT, o);
+        else oy.template store<false>(rows_at(y), sq, len - t0, o);
+        y += adv * yt;
     }
     if (SUMMARY) {
         if (d < a.D) {
             const long long at_ = ((long long)c * a.B + b) * a.D + d;
-            *reinterpret_cast<float4*>(a.runs + at_ * NP + nq * 4) = f4(h);
+            store_pack<float, NS>(a.runs + at_ * NP + nq * NS, h);
             if (nq == 0) a.runs_dt[at_] = dsum;
         }
         return;
     }
-    // tiles without a valid frame: outputs 0, the state in front of them for the backward pass
-    S* y = static_cast<S*>(a.y) + (long long)b * a.D + sd;
-    for (; t0 < p1; t0 += TT) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            if (chan && p < p1) y[(long long)p * a.B * a.D] = (S)0.f;
-        }
-    }
-    if (a.h_out && d < a.D && c == a.nrun - 1) store_states(a.h_out + ((long long)b * a.D + d) * a.N, nq * 4, a.N, h);
+    S* y0 = static_cast<S*>(a.y) + (long long)b * a.D + sd;
+    for (int p = max(stop, p0) + sq; p < p1; p += 256 / CB)          // frames behind the clip's end
+        if (chan) y0[p * yt] = (S)0.f;
+    if (a.h_out && d < a.D && c == a.nrun - 1) store_states<NS>(a.h_out + ((long long)b * a.D + d) * a.N, nq * NS, a.N, h);
 }
 
 // ------------------------------------------------------------------------------------------------ backward
 // adjoint from behind a run: what the run's own dy leave on the state in front of it (runs), and its sum of D
-template <class S, int LN>
+template <class S, int LN, int NS>
 __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
-    constexpr int NP = 4 * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4, NBC = (TT * NP + 255) / 256;
+    constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4;
+    using Rows = LaneRows<S, 4>;
+    using BC = StateRows<S, TT, NP>;
     __shared__ __attribute__((aligned(16))) float sD[2][CB * LD], sG[2][CB * LD], sC[2][TT * NP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     const int ch = wave * (64 / LN) + lane / LN;
-    const int b = blockIdx.y, c = blockIdx.z + 1, d = blockIdx.x * CB + ch;          // run 0 has nothing in front of it
-    const int sch = tid % CB, sq = tid / CB, sd = blockIdx.x * CB + sch;
-    const bool chan = sd < a.D;
+    const ScanBlock blk = scan_block<S, CB>();
+    const int b = blk.b, c = blk.c + 1, d0 = blk.x * CB, d = d0 + ch;         // run 0 has nothing in front of it
+    const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;
+    const bool chan = sd < a.D, gated = a.z != nullptr;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
     const int p0 = c * a.run, stop = min(min(p0 + a.run, a.T), len);
-    const S* e = static_cast<const S*>(a.delta) + b * a.eb + sd;
-    const S* z = static_cast<const S*>(a.z) + b * a.zb + sd;
-    const S* g = static_cast<const S*>(a.dy) + b * a.gb + sd;
-    const S* cm = static_cast<const S*>(a.c) + b * a.cb;
-    auto frame = [&](int p) { return (long long)(a.reverse && p < len ? len - 1 - p : p); };
-    const float bias = chan && a.dbias ? a.dbias[sd] : 0.f;
-    float A2[4], r[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) A2[j] = d < a.D && nq * 4 + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * 4 + j]) : 0.f;
-    float re[4], rz[4], rg[4], rc[NBC];
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            const bool on = chan && p < len;
-            const long long f = frame(p);
-            re[i] = on ? (float)e[f * a.et] : 0.f;
-            rz[i] = on && a.z ? (float)z[f * a.zt] : 0.f;
-            rg[i] = on ? (float)g[f * a.gt] : 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k, p = t0 + i / NP, n = i % NP;
-            rc[k] = i < TT * NP && p < len && n < a.N ? (float)cm[frame(p) * a.ct + n] : 0.f;
-        }
-    };
     int buf = 0, t0 = p0 + (stop > p0 ? (stop - p0 - 1) / TT * TT : -TT);
-    if (t0 >= p0) fetch(t0);
+    const long long f0 = a.reverse ? (long long)len - t0 - TT : t0, adv = a.reverse ? TT : -TT;
+    const S* e = static_cast<const S*>(a.delta) + b * a.eb + d0 + f0 * a.et;
+    const S* z = static_cast<const S*>(a.z) + b * a.zb + d0 + f0 * a.zt;
+    const S* g = static_cast<const S*>(a.dy) + b * a.gb + d0 + f0 * a.gt;
+    const S* cm = static_cast<const S*>(a.c) + b * a.cb + f0 * a.ct;
+    const Rows oe(a.et, TT, sq, sch, a.reverse, chan), oz(a.zt, TT, sq, sch, a.reverse, chan & gated), og(a.gt, TT, sq, sch, a.reverse, chan);
+    const BC oc(a.ct, a.N, a.reverse);
+    const float bias = chan && a.dbias ? a.dbias[sd] : 0.f;
+    float A2[NS], r[NS] = {}, dsum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) A2[j] = d < a.D && nq * NS + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
+    arrived(A2);
+    float re[4], rz[4], rg[4], rc[BC::NB];
+    auto request = [&](auto full, int left) __attribute__((always_inline)) {
+        oe.template load<full()>(rows_at(e), sq, left, re);
+        oz.template load<full()>(rows_at(z), sq, left, rz);
+        og.template load<full()>(rows_at(g), sq, left, rg);
+        oc.template load<full()>(rows_at(cm), left, rc);
+    };
+    auto fetch = [&](int left) __attribute__((always_inline)) {
+        if (left >= TT) request(std::true_type(), left);
+        else request(std::false_type(), left);
+        e += adv * a.et; z += adv * a.zt; g += adv * a.gt; cm += adv * a.ct;
+    };
+    if (t0 >= p0) fetch(len - t0);
     for (; t0 >= p0; t0 -= TT, buf ^= 1) {
         float D4[4], G4[4];
+        steps_of<4>(a, re, bias, sq * 4, len - t0, D4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = t0 + sq * 4 + i;
-            D4[i] = chan && p < len ? step_of(a, re[i] + bias) : 0.f;
-            G4[i] = a.z ? rg[i] * (rz[i] * fast_sigmoid(rz[i])) : rg[i];
-        }
-        *reinterpret_cast<float4*>(&sD[buf][sch * LD + sq * 4]) = f4(D4);
-        *reinterpret_cast<float4*>(&sG[buf][sch * LD + sq * 4]) = f4(G4);
+        for (int i = 0; i < 4; ++i) G4[i] = rg[i];
+        if (a.z)
 #pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k;
-            if (i < TT * NP) sC[buf][i] = rc[k];
-        }
+            for (int i = 0; i < 4; ++i) G4[i] *= rz[i] * fast_sigmoid(rz[i]);
+        store_pack<float, 4>(&sD[buf][sch * LD + sq * 4], D4);
+        store_pack<float, 4>(&sG[buf][sch * LD + sq * 4], G4);
+        oc.put(sC[buf], rc);
         __syncthreads();
-        if (t0 - TT >= p0) fetch(t0 - TT);
+        if (t0 - TT >= p0) fetch(len - t0 + TT);
+        const float *rowD = &sD[buf][ch * LD], *rowG = &sG[buf][ch * LD];
+        ScanGroup<NS, false> gr;                                 // (D, g, C in the places of D, U, B)
+        gr.template load<NP>(rowD, rowG, sC[buf], nullptr, TT / 4 - 1, nq);
 #pragma unroll
         for (int q = TT / 4 - 1; q >= 0; --q) {
-            const float4 dt4 = *reinterpret_cast<const float4*>(&sD[buf][ch * LD + 4 * q]), g4 = *reinterpret_cast<const float4*>(&sG[buf][ch * LD + 4 * q]);
+            ScanGroup<NS, false> next;
+            if (q) next.template load<NP>(rowD, rowG, sC[buf], nullptr, q - 1, nq);
+            __builtin_amdgcn_sched_barrier(0);
+            float ex[4][NS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) ex[i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
-                const float4 Cv = *reinterpret_cast<const float4*>(&sC[buf][(4 * q + i) * NP + nq * 4]);
-                const float dt = at(dt4, i), gi = at(g4, i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = fmaf(at(Cv, j), gi, r[j]) * __builtin_amdgcn_exp2f(dt * A2[j]);
-                dsum += dt;
+                for (int j = 0; j < NS; ++j) r[j] = fmaf(gr.B[i].v[j], at(gr.U, i), r[j]) * ex[i][j];
+                dsum += at(gr.D, i);
             }
+            if (q) gr = next;
         }
     }
     if (d < a.D) {
         const long long at_ = ((long long)c * a.B + b) * a.D + d;
-        *reinterpret_cast<float4*>(a.runs + at_ * NP + nq * 4) = f4(r);
+        store_pack<float, NS>(a.runs + at_ * NP + nq * NS, r);
         if (nq == 0) a.runs_dt[at_] = dsum;
     }
 }
 
-// Sums of eight values per lane (four states: dB, dC) over the wave's lanes with the same nq.  Halving the number of values at
-// every step while the lanes that hold them spread out (v_permlane32_swap / v_permlane16_swap exchange halves of a register pair),
-// so eight sums over 64 / LN lanes cost 17 instructions for LN = 4 instead of 8 x 8.  Afterwards a lane holds dB (lane < 32) or dC of
-// state 4 nq + 2 (lane >> 4 & 1) + (lane >> 3 & 1) in v0 (LN = 16: of states 4 nq + 2 (lane >> 4 & 1) + 0 and + 1 in v0, v1).
+// Sums of 2 NS values per lane (dB, dC of its states) over the wave's lanes with the same nq.  Every step halves the number of values
+// while the lanes that hold them spread out (v_permlane32_swap / v_permlane16_swap exchange halves of a register pair): the four sums
+// over the 8 channels of LN = 8 cost 7 instructions instead of 4 x 3 (with moves).  Afterwards a lane holds dB (lane < 32) or dC of state
+// NS nq + (lane >> 4 & 1) in v[0]; NS = 4: of states 4 nq + 2 (lane >> 4 & 1) + 0, 1 in v[0], v[1].
 __device__ __forceinline__ float swap_add32(float x, float y) {      // lanes < 32: x.lo + x.hi, lanes >= 32: y.lo + y.hi
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
@@ -304,241 +467,274 @@ __device__ __forceinline__ float swap_add16(float x, float y) {      // even 16-
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-template <int LN>
-__device__ __forceinline__ void channel_sums(const float (&vB)[4], const float (&vC)[4], int lane, float& v0, float& v1) {
-    float w[4];
+template <int LN, int NS>
+__device__ __forceinline__ void channel_sums(const float (&vB)[NS], const float (&vC)[NS], float (&v)[NS / 2]) {
+    float w[NS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = swap_add32(vB[j], vC[j]);
-    const float x0 = swap_add16(w[0], w[2]), x1 = swap_add16(w[1], w[3]);
-    if constexpr (LN == 16) { v0 = x0; v1 = x1; return; }
-    const bool up = lane & 8;
-    float v = (up ? x1 : x0) + dpp_shuffled<0x128>(up ? x0 : x1);    // row_ror:8 = lane ^ 8
-    if constexpr (LN <= 4) v += dpp_shuffled<0x1B>(dpp_shuffled<0x141>(v));      // lane ^ 4: half mirror (^ 7), then quad reversal (^ 3)
-    if constexpr (LN <= 2) v += dpp_shuffled<0x4E>(v);
-    if constexpr (LN <= 1) v += dpp_shuffled<0xB1>(v);
-    v0 = v;
-    v1 = 0.f;
+    for (int j = 0; j < NS; ++j) w[j] = swap_add32(vB[j], vC[j]);
+#pragma unroll
+    for (int j = 0; j < NS / 2; ++j) {
+        v[j] = swap_add16(w[j], w[j + NS / 2]);
+        if constexpr (LN <= 8) v[j] += dpp_lane<0x128>(v[j]);                            // row_ror:8 = lane ^ 8
+        if constexpr (LN <= 4) v[j] += dpp_lane<0x1B>(dpp_lane<0x141>(v[j]));            // lane ^ 4: half mirror (^ 7), then quad reversal (^ 3)
+    }
 }
 
 // grid (channel blocks, B, runs).  Tiles of 16 frames from the back: the tile's states are recomputed from the saved state in front of
-// it and kept in registers (q_t = exp(D_t A) h_{t-1} and the exponential itself), then the adjoint runs back over them.
-template <class S, int LN>
+// it and kept in registers (q_t = exp(D_t A) h_{t-1} and the exponential itself), then the adjoint runs back over them.  What a thread
+// needs again when the tile's sums are known (D, u, sigmoid(raw), g, dy silu'(z) of its four frames) waits in its own corner of LDS.
+template <int LN, int NS> struct ScanBwdLds {
+    static constexpr int NP = NS * LN, CB = 256 / LN, TT = SC_SAVE, LD = TT + 4, F = CB * TT / 256;
+    static constexpr int rows = CB * LD, bc = TT * NP, part = 4 * TT * 2 * NP, keep = 5 * 256 * F;
+    static constexpr size_t bytes = (size_t)(3 * rows + 2 * bc + part + keep) * sizeof(float);
+};
+template <class S, int LN, int NS>
 __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(ScanArgs a) {
-    constexpr int NP = 4 * LN, CB = 256 / LN, TT = SC_SAVE, LD = TT + 4, ITEMS = CB * TT / 4, IT = (ITEMS + 255) / 256;
-    constexpr int NBC = (TT * NP + 255) / 256;
+    using L = ScanBwdLds<LN, NS>;
+    constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F;                  // F frames of a channel per thread and tile
+    constexpr int NP2 = TT * 2 * NP / 256;
+    using Rows = LaneRows<S, F>;
+    using BC = StateRows<S, TT, NP>;
+    static_assert(F >= 1 && NP2 >= 1 && L::rows >= 256, "a tile has work for every thread");
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    float *sD = smem, *sU = sD + CB * LD, *sG = sU + CB * LD, *sB = sG + CB * LD, *sC = sB + TT * NP, *sP = sC + TT * NP;   // sP [4][TT][2 NP]
+    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *sB = sG + L::rows, *sC = sB + L::bc, *sP = sC + L::bc;     // sP [4][TT][2 NP]
+    Pack<float, F>* keep = reinterpret_cast<Pack<float, F>*>(sP + L::part) + threadIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     const int ch = wave * (64 / LN) + lane / LN;
-    const int b = blockIdx.y, c = blockIdx.z, d = blockIdx.x * CB + ch;
+    const ScanBlock blk = scan_block<S, CB>();
+    const int b = blk.b, c = blk.c, d0 = blk.x * CB, d = d0 + ch;
+    const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;      // staging: channel, group of F frames
+    const bool chan = sd < a.D, gated = a.z != nullptr;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
     const int p0 = c * a.run, p1 = min(p0 + a.run, a.T), stop = min(p1, len);
-    const S* u = static_cast<const S*>(a.u) + b * a.ub;
-    const S* e = static_cast<const S*>(a.delta) + b * a.eb;
-    const S* z = static_cast<const S*>(a.z) + b * a.zb;
-    const S* g = static_cast<const S*>(a.dy) + b * a.gb;
-    const S* bm = static_cast<const S*>(a.b) + b * a.bb;
-    const S* cm = static_cast<const S*>(a.c) + b * a.cb;
-    S* du = static_cast<S*>(a.du) + (long long)b * a.D;
-    S* de = static_cast<S*>(a.ddelta) + (long long)b * a.D;
-    S* dz = static_cast<S*>(a.dz) + b * a.dzb;
-    const long long row = (long long)a.B * a.D;
-    auto frame = [&](int p) { return (long long)(a.reverse && p < len ? len - 1 - p : p); };
-    // staging items: (channel, group of four frames)
-    float bias[IT], skip[IT], dskip[IT], dbias[IT];
+    int t0 = p0 + (stop > p0 ? (stop - p0 - 1) / TT * TT : -TT);
+    const long long f0 = a.reverse ? (long long)len - t0 - TT : t0, adv = a.reverse ? TT : -TT, row = (long long)a.B * a.D;
+    const S* u = static_cast<const S*>(a.u) + b * a.ub + d0 + f0 * a.ut;
+    const S* e = static_cast<const S*>(a.delta) + b * a.eb + d0 + f0 * a.et;
+    const S* z = static_cast<const S*>(a.z) + b * a.zb + d0 + f0 * a.zt;
+    const S* g = static_cast<const S*>(a.dy) + b * a.gb + d0 + f0 * a.gt;
+    const S* bm = static_cast<const S*>(a.b) + b * a.bb + f0 * a.bt;
+    const S* cm = static_cast<const S*>(a.c) + b * a.cb + f0 * a.ct;
+    const float* hm = a.saved + (((long long)(t0 / TT) * a.B + b) * a.D + d0) * NP;
+    S* du = static_cast<S*>(a.du) + (long long)b * a.D + d0 + f0 * row;
+    S* de = static_cast<S*>(a.ddelta) + (long long)b * a.D + d0 + f0 * row;
+    S* dz = static_cast<S*>(a.dz) + b * a.dzb + d0 + f0 * a.dzt;
+    float* bc = a.bc + (((long long)blk.x * a.T + f0) * a.B + b) * 2 * NP;
+    const Rows ou(a.ut, TT, sq, sch, a.reverse, chan), oe(a.et, TT, sq, sch, a.reverse, chan), og(a.gt, TT, sq, sch, a.reverse, chan);
+    const Rows oz(a.zt, TT, sq, sch, a.reverse, chan & gated), oo(row, TT, sq, sch, a.reverse, chan), ow(a.dzt, TT, sq, sch, a.reverse, chan & gated);
+    const BC ob(a.bt, a.N, a.reverse), oc(a.ct, a.N, a.reverse);
+    const unsigned oh = d < a.D ? (unsigned)((ch * NP + nq * NS) * 4) : SC_OUT;
+    unsigned op[NP2];
 #pragma unroll
-    for (int k = 0; k < IT; ++k) {
-        const int i = tid + 256 * k, sd = blockIdx.x * CB + i % CB;
-        const bool on = i < ITEMS && sd < a.D;
-        bias[k] = on && a.dbias ? a.dbias[sd] : 0.f;
-        skip[k] = on && a.skip ? a.skip[sd] : 0.f;
-        dskip[k] = dbias[k] = 0.f;
+    for (int k = 0; k < NP2; ++k) {
+        const int i = tid + 256 * k, m = i / (2 * NP);
+        op[k] = ((unsigned)(a.reverse ? TT - 1 - m : m) * (unsigned)(a.B * 2 * NP) + (unsigned)(i % (2 * NP))) * 4u;
     }
-    float A2[4], A[4], r[4] = {0.f, 0.f, 0.f, 0.f}, da[4] = {0.f, 0.f, 0.f, 0.f};
+    const float bias = chan && a.dbias ? a.dbias[sd] : 0.f, skip = chan && a.skip ? a.skip[sd] : 0.f;
+    float dskip = 0.f, dbias = 0.f;
+    float A2[NS], A[NS], r[NS] = {}, da[NS] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        A[j] = d < a.D && nq * 4 + j < a.N ? -rate_of(a.a_log[(long long)d * a.N + nq * 4 + j]) : 0.f;
+    for (int j = 0; j < NS; ++j) {
+        A[j] = d < a.D && nq * NS + j < a.N ? -rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
         A2[j] = A[j] * LOG2E;
     }
     if (d < a.D) {
-        if (a.dh_out) load_states(a.dh_out + ((long long)b * a.D + d) * a.N, nq * 4, a.N, r);
-        fold_runs<LN>(a, a.nrun - 1, c, -1, b, d, nq, A2, r);
+        if (a.dh_out) load_states<NS>(a.dh_out + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
+        if (a.nrun > 1) fold_runs<LN, NS>(a, c, a.nrun - 1, c, -1, b, d, nq, A2, r);
     }
-    float ru[IT][4], re[IT][4], rz[IT][4], rg[IT][4], rb[NBC], rc[NBC];
-    float4 rh = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int i = tid + 256 * k, sd = blockIdx.x * CB + i % CB, sq = i / CB;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int p = t0 + sq * 4 + m;
-                const bool on = i < ITEMS && sd < a.D && p < len;
-                const long long f = frame(p);
-                ru[k][m] = on ? (float)u[f * a.ut + sd] : 0.f;
-                re[k][m] = on ? (float)e[f * a.et + sd] : 0.f;
-                rz[k][m] = on && a.z ? (float)z[f * a.zt + sd] : 0.f;
-                rg[k][m] = on ? (float)g[f * a.gt + sd] : 0.f;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k, p = t0 + i / NP, n = i % NP;
-            const bool on = i < TT * NP && p < len && n < a.N;
-            rb[k] = on ? (float)bm[frame(p) * a.bt + n] : 0.f;
-            rc[k] = on ? (float)cm[frame(p) * a.ct + n] : 0.f;
-        }
-        if (d < a.D) rh = *reinterpret_cast<const float4*>(a.saved + (((long long)(t0 / TT) * a.B + b) * a.D + d) * NP + nq * 4);
-    };
     // frames behind the clip's end: gradients 0
-    for (int p = max(stop, p0) + tid / CB; p < p1; p += 256 / CB) {
-        const int sd = blockIdx.x * CB + tid % CB;
-        if (sd < a.D) {
-            du[p * row + sd] = (S)0.f;
-            de[p * row + sd] = (S)0.f;
-            if (a.z) dz[p * a.dzt + sd] = (S)0.f;
+    for (int p = max(stop, p0) + sq; p < p1; p += 256 / CB)
+        if (chan) {
+            static_cast<S*>(a.du)[p * row + (long long)b * a.D + sd] = (S)0.f;
+            static_cast<S*>(a.ddelta)[p * row + (long long)b * a.D + sd] = (S)0.f;
+            if (gated) static_cast<S*>(a.dz)[p * a.dzt + b * a.dzb + sd] = (S)0.f;
         }
-    }
     for (long long i = tid; i < (long long)(p1 - max(stop, p0)) * 2 * NP; i += 256)
-        a.bc[(((long long)blockIdx.x * a.T + max(stop, p0) + i / (2 * NP)) * a.B + b) * 2 * NP + i % (2 * NP)] = 0.f;
+        a.bc[(((long long)blk.x * a.T + max(stop, p0) + i / (2 * NP)) * a.B + b) * 2 * NP + i % (2 * NP)] = 0.f;
+    arrived(r);
 
-    int t0 = p0 + (stop > p0 ? (stop - p0 - 1) / TT * TT : -TT);
-    if (t0 >= p0) fetch(t0);
+    float ru[F], re[F], rz[F], rg[F], rb[BC::NB], rc[BC::NB], rh[NS];
+    auto request = [&](auto full, int left) __attribute__((always_inline)) {
+        ou.template load<full()>(rows_at(u), sq, left, ru);
+        oe.template load<full()>(rows_at(e), sq, left, re);
+        oz.template load<full()>(rows_at(z), sq, left, rz);
+        og.template load<full()>(rows_at(g), sq, left, rg);
+        ob.template load<full()>(rows_at(bm), left, rb);
+        oc.template load<full()>(rows_at(cm), left, rc);
+    };
+    auto fetch = [&](int left) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) rh[j] = row_load<float>(rows_at(hm), oh, 4 * j);
+        if (left >= TT) request(std::true_type(), left);
+        else request(std::false_type(), left);
+        u += adv * a.ut; e += adv * a.et; z += adv * a.zt; g += adv * a.gt; bm += adv * a.bt; cm += adv * a.ct;
+        hm -= row * NP;
+    };
+    if (t0 >= p0) {
+        fetch(len - t0);
+#pragma unroll
+        for (int i = 0; i < 3 * F + NP2; ++i) row_store<S>(0.f, rows_at(du), SC_OUT, 4 * i);       // (see scan_fwd_kernel)
+    }
     for (; t0 >= p0; t0 -= TT) {
-        float cu[IT][4], ce[IT][4], cz[IT][4], cg[IT][4];
+        float D4[F], U4[F], S4[F], G4[F], Z4[F];
+        steps_of<F>(a, re, bias, sq * F, len - t0, D4);
 #pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int i = tid + 256 * k, sch = i % CB, sd = blockIdx.x * CB + sch, sq = i / CB;
-            float D4[4], U4[4], G4[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                cu[k][m] = ru[k][m]; ce[k][m] = re[k][m] + bias[k]; cz[k][m] = rz[k][m]; cg[k][m] = rg[k][m];
-                D4[m] = sd < a.D && t0 + sq * 4 + m < len ? step_of(a, ce[k][m]) : 0.f;
-                U4[m] = D4[m] * cu[k][m];
-                G4[m] = a.z ? cg[k][m] * (cz[k][m] * fast_sigmoid(cz[k][m])) : cg[k][m];
-            }
-            if (i < ITEMS) {
-                *reinterpret_cast<float4*>(&sD[sch * LD + sq * 4]) = f4(D4);
-                *reinterpret_cast<float4*>(&sU[sch * LD + sq * 4]) = f4(U4);
-                *reinterpret_cast<float4*>(&sG[sch * LD + sq * 4]) = f4(G4);
-            }
+        for (int i = 0; i < F; ++i) {
+            S4[i] = fast_sigmoid(re[i] + bias);
+            U4[i] = D4[i] * ru[i];
+            G4[i] = rg[i];
+            Z4[i] = 0.f;
         }
+        if (!a.softplus)
 #pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int i = tid + 256 * k;
-            if (i < TT * NP) { sB[i] = rb[k]; sC[i] = rc[k]; }
-        }
-        float h[4] = {rh.x, rh.y, rh.z, rh.w};
+            for (int i = 0; i < F; ++i) S4[i] = 1.f;
+        if (a.z)
+#pragma unroll
+            for (int i = 0; i < F; ++i) {
+                const float sg = fast_sigmoid(rz[i]);
+                G4[i] = rg[i] * (rz[i] * sg);
+                Z4[i] = rg[i] * (sg * fmaf(rz[i], 1.f - sg, 1.f));
+            }
+#pragma unroll
+        for (int i = 0; i < F; ++i) dskip = fmaf(G4[i], ru[i], dskip);
+        store_pack<float, F>(sD + sch * LD + sq * F, D4);
+        store_pack<float, F>(sU + sch * LD + sq * F, U4);
+        store_pack<float, F>(sG + sch * LD + sq * F, G4);
+        store_pack<float, F>(keep[0].v, D4);
+        store_pack<float, F>(keep[256].v, ru);
+        store_pack<float, F>(keep[512].v, S4);
+        store_pack<float, F>(keep[768].v, G4);
+        store_pack<float, F>(keep[1024].v, Z4);
+        ob.put(sB, rb);
+        oc.put(sC, rc);
+        float h[NS];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) h[j] = rh[j];
         __syncthreads();
-        if (t0 - TT >= p0) fetch(t0 - TT);
+        if (t0 - TT >= p0) fetch(len - t0 + TT);
         float *rowD = sD + ch * LD, *rowU = sU + ch * LD, *rowG = sG + ch * LD;
-        float ex[TT][4], q[TT][4];
+        float ex[TT][NS], q[TT][NS];
+        ScanGroup<NS, false> gr;
+        gr.template load<NP>(rowD, rowU, sB, nullptr, 0, nq);
 #pragma unroll
         for (int k = 0; k < TT / 4; ++k) {
-            const float4 dt4 = *reinterpret_cast<const float4*>(rowD + 4 * k), du4 = *reinterpret_cast<const float4*>(rowU + 4 * k);
+            ScanGroup<NS, false> next;
+            if (k + 1 < TT / 4) next.template load<NP>(rowD, rowU, sB, nullptr, k + 1, nq);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 Bv = *reinterpret_cast<const float4*>(&sB[(4 * k + i) * NP + nq * 4]);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(dt4, i) * A2[j]);
+                for (int j = 0; j < NS; ++j) ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
                     q[4 * k + i][j] = ex[4 * k + i][j] * h[j];
-                    h[j] = fmaf(at(du4, i), at(Bv, j), q[4 * k + i][j]);
+                    h[j] = fmaf(at(gr.U, i), gr.B[i].v[j], q[4 * k + i][j]);
                 }
-            }
+            if (k + 1 < TT / 4) gr = next;
         }
-        float dat[4] = {0.f, 0.f, 0.f, 0.f};
+        float dat[NS] = {};
+        ScanGroup<NS, true> gb;
+        float4 g4 = *reinterpret_cast<const float4*>(rowG + TT - 4);
+        gb.template load<NP>(rowD, rowU, sB, sC, TT / 4 - 1, nq);
 #pragma unroll
         for (int k = TT / 4 - 1; k >= 0; --k) {
-            const float4 dt4 = *reinterpret_cast<const float4*>(rowD + 4 * k), du4 = *reinterpret_cast<const float4*>(rowU + 4 * k);
-            const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
+            ScanGroup<NS, true> next;
+            float4 gn = g4;
+            if (k) {
+                next.template load<NP>(rowD, rowU, sB, sC, k - 1, nq);
+                gn = *reinterpret_cast<const float4*>(rowG + 4 * (k - 1));
+            }
+            __builtin_amdgcn_sched_barrier(0);
             float yo[4], bo[4], ko[4];
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
                 const int s = 4 * k + i;
-                const float4 Bv = *reinterpret_cast<const float4*>(&sB[s * NP + nq * 4]), Cv = *reinterpret_cast<const float4*>(&sC[s * NP + nq * 4]);
-                const float dt = at(dt4, i), dui = at(du4, i), gi = at(g4, i);
-                float y = 0.f, rbs = 0.f, ks = 0.f, vB[4], vC[4];
+                const float dt = at(gb.D, i), dui = at(gb.U, i), gi = at(g4, i);
+                float vB[NS], vC[NS], v[NS / 2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float rj = fmaf(at(Cv, j), gi, r[j]), hj = fmaf(dui, at(Bv, j), q[s][j]), rq = rj * q[s][j];
-                    y = fmaf(at(Cv, j), hj, y);
-                    rbs = fmaf(at(Bv, j), rj, rbs);
-                    ks = fmaf(A[j], rq, ks);
+                for (int j = 0; j < NS; ++j) {
+                    const float rj = fmaf(gb.Cv[i].v[j], gi, r[j]), hj = fmaf(dui, gb.B[i].v[j], q[s][j]), rq = rj * q[s][j];
+                    yo[i] = j ? fmaf(gb.Cv[i].v[j], hj, yo[i]) : gb.Cv[i].v[j] * hj;
+                    bo[i] = j ? fmaf(gb.B[i].v[j], rj, bo[i]) : gb.B[i].v[j] * rj;
+                    ko[i] = j ? fmaf(A[j], rq, ko[i]) : A[j] * rq;
                     dat[j] = fmaf(dt, rq, dat[j]);
                     vB[j] = rj * dui;
                     vC[j] = gi * hj;
                     r[j] = rj * ex[s][j];
                 }
-                yo[i] = lanes_sum<LN>(y);
-                bo[i] = lanes_sum<LN>(rbs);
-                ko[i] = lanes_sum<LN>(ks);
-                float v0, v1;
-                channel_sums<LN>(vB, vC, lane, v0, v1);
-                float* o = sP + (wave * TT + s) * 2 * NP + (lane >> 5) * NP + nq * 4 + 2 * ((lane >> 4) & 1);
-                if constexpr (LN == 16) { o[0] = v0; o[1] = v1; }
-                else o[(lane >> 3) & 1] = v0;
+                channel_sums<LN, NS>(vB, vC, v);
+                float* o = sP + (wave * TT + s) * 2 * NP + (lane >> 5) * NP + nq * NS + ((lane >> 4) & 1) * (NS / 2);
+#pragma unroll
+                for (int j = 0; j < NS / 2; ++j) o[j] = v[j];
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                yo[i] = lanes_sum<LN>(yo[i]);
+                bo[i] = lanes_sum<LN>(bo[i]);
+                ko[i] = lanes_sum<LN>(ko[i]);
+            }
+            arrived(yo);
+            arrived(bo);
+            arrived(ko);
             if (nq == 0) {                                       // the channel's lanes have read these four frames
-                *reinterpret_cast<float4*>(rowD + 4 * k) = f4(ko);
-                *reinterpret_cast<float4*>(rowU + 4 * k) = f4(bo);
-                *reinterpret_cast<float4*>(rowG + 4 * k) = f4(yo);
+                store_pack<float, 4>(rowD + 4 * k, ko);
+                store_pack<float, 4>(rowU + 4 * k, bo);
+                store_pack<float, 4>(rowG + 4 * k, yo);
             }
+            if (k) { gb = next; g4 = gn; }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) da[j] += dat[j];
+        for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (sums over a tile first: long clips keep their digits)
         __syncthreads();
+        const Pack<float, F> kk = *reinterpret_cast<const Pack<float, F>*>(sD + sch * LD + sq * F), bb = *reinterpret_cast<const Pack<float, F>*>(sU + sch * LD + sq * F);
+        const Pack<float, F> yy = *reinterpret_cast<const Pack<float, F>*>(sG + sch * LD + sq * F);
+        const Pack<float, F> kD = keep[0], ku = keep[256], kS = keep[512], kG = keep[768], kZ = keep[1024];
+        float tile_bias = 0.f, xu[F], xe[F], xz[F];
 #pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int i = tid + 256 * k, sch = i % CB, sd = blockIdx.x * CB + sch, sq = i / CB;
-            if (i < ITEMS && sd < a.D) {
-                const float4 k4 = *reinterpret_cast<const float4*>(&sD[sch * LD + sq * 4]), b4 = *reinterpret_cast<const float4*>(&sU[sch * LD + sq * 4]);
-                const float4 y4 = *reinterpret_cast<const float4*>(&sG[sch * LD + sq * 4]);
+        for (int i = 0; i < F; ++i) {
+            xe[i] = fmaf(ku.v[i], bb.v[i], kk.v[i]) * kS.v[i];
+            xu[i] = fmaf(kG.v[i], skip, kD.v[i] * bb.v[i]);
+            xz[i] = kZ.v[i] * fmaf(skip, ku.v[i], yy.v[i]);
+            tile_bias += sq * F + i < len - t0 ? xe[i] : 0.f;
+        }
+        dbias += tile_bias;
+        float v[NP2];
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const int p = t0 + sq * 4 + m;
-                    if (p >= stop) continue;
-                    const long long f = frame(p);
-                    const float dt = step_of(a, ce[k][m]), sz = a.z ? fast_sigmoid(cz[k][m]) : 1.f;
-                    const float gi = a.z ? cg[k][m] * (cz[k][m] * sz) : cg[k][m];
-                    const float dd = fmaf(cu[k][m], at(b4, m), at(k4, m)) * (a.softplus ? fast_sigmoid(ce[k][m]) : 1.f);
-                    du[f * row + sd] = (S)fmaf(gi, skip[k], dt * at(b4, m));
-                    de[f * row + sd] = (S)dd;
-                    if (a.z) dz[f * a.dzt + sd] = (S)(cg[k][m] * fmaf(skip[k], cu[k][m], at(y4, m)) * sz * fmaf(cz[k][m], 1.f - sz, 1.f));
-                    dskip[k] = fmaf(gi, cu[k][m], dskip[k]);
-                    dbias[k] += dd;
-                }
-            }
+        for (int k = 0; k < NP2; ++k) {
+            const int i = tid + 256 * k;
+            v[k] = (sP[i] + sP[TT * 2 * NP + i]) + (sP[2 * TT * 2 * NP + i] + sP[3 * TT * 2 * NP + i]);
         }
-        for (int i = tid; i < TT * 2 * NP; i += 256) {
-            const int p = t0 + i / (2 * NP);
-            if (p < stop)
-                a.bc[(((long long)blockIdx.x * a.T + frame(p)) * a.B + b) * 2 * NP + i % (2 * NP)] =
-                    (sP[i] + sP[TT * 2 * NP + i]) + (sP[2 * TT * 2 * NP + i] + sP[3 * TT * 2 * NP + i]);
-        }
+        auto write = [&](auto full, int left) __attribute__((always_inline)) {
+            oo.template store<full()>(rows_at(du), sq, left, xu);
+            oo.template store<full()>(rows_at(de), sq, left, xe);
+            ow.template store<full()>(rows_at(dz), sq, left, xz);
+#pragma unroll
+            for (int k = 0; k < NP2; ++k) row_store<float>(v[k], rows_at(bc), full() || (tid + 256 * k) / (2 * NP) < left ? op[k] : SC_OUT, 0);
+        };
+        if (len - t0 >= TT) write(std::true_type(), TT);
+        else write(std::false_type(), len - t0);
+        du += adv * row; de += adv * row; dz += adv * a.dzt; bc += adv * a.B * 2 * NP;
         __syncthreads();                                         // before the next tile is staged
     }
-    if (a.dh0 && d < a.D && c == 0) store_states(a.dh0 + ((long long)b * a.D + d) * a.N, nq * 4, a.N, r);
+    if (a.dh0 && d < a.D && c == 0) store_states<NS>(a.dh0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
     if (!a.sums) return;
     float* out = a.sums + ((long long)c * a.B + b) * ((long long)a.D * (a.N + 2));
     if (d < a.D) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (nq * 4 + j < a.N) out[(long long)d * a.N + nq * 4 + j] = A[j] * da[j];
+        for (int j = 0; j < NS; ++j)
+            if (nq * NS + j < a.N) out[(long long)d * a.N + nq * NS + j] = A[j] * da[j];
     }
-    // the four groups of frames of a channel meet in LDS
-#pragma unroll
-    for (int k = 0; k < IT; ++k) {
-        const int i = tid + 256 * k;
-        if (i < ITEMS) { sD[i] = dskip[k]; sU[i] = dbias[k]; }
-    }
+    // the groups of frames of a channel meet in LDS
+    sD[tid] = dskip;
+    sU[tid] = dbias;
     __syncthreads();
-    for (int i = tid; i < CB; i += 256) {
-        const int sd = blockIdx.x * CB + i;
-        if (sd < a.D) {
-            out[(long long)a.D * a.N + sd] = (sD[i] + sD[CB + i]) + (sD[2 * CB + i] + sD[3 * CB + i]);
-            out[(long long)a.D * (a.N + 1) + sd] = (sU[i] + sU[CB + i]) + (sU[2 * CB + i] + sU[3 * CB + i]);
-        }
+    if (tid < CB && chan) {
+        float s0 = sD[tid], s1 = sU[tid];
+        for (int k = 1; k < 256 / CB; ++k) { s0 += sD[tid + k * CB]; s1 += sU[tid + k * CB]; }
+        out[(long long)a.D * a.N + sd] = s0;
+        out[(long long)a.D * (a.N + 1) + sd] = s1;
     }
 }
 
@@ -563,34 +759,34 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* bc, S* db, S
 
 // ------------------------------------------------------------------------------------------------ one frame
 // u, delta, z [B][D] and b, c [B][N] at clip strides, state [B][D][N] float -> state_out (which may be the same memory)
-template <class S, int LN>
+template <class S, int LN, int NS>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     constexpr int CB = 256 / LN;
     const int nq = threadIdx.x % LN, b = blockIdx.y, dd = blockIdx.x * CB + threadIdx.x / LN;
     const bool on = dd < a.D;
     const int d = on ? dd : 0;                                   // (every lane takes part in the sum)
     const long long s0 = ((long long)b * a.D + d) * a.N;
-    float h[4], al[4], Bv[4], Cv[4];
-    load_states(a.h0 + s0, nq * 4, a.N, h);
-    load_states(a.a_log + (long long)d * a.N, nq * 4, a.N, al);
+    float h[NS], al[NS], Bv[NS], Cv[NS];
+    load_states<NS>(a.h0 + s0, nq * NS, a.N, h);
+    load_states<NS>(a.a_log + (long long)d * a.N, nq * NS, a.N, al);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool has = nq * 4 + j < a.N;
-        Bv[j] = has ? (float)static_cast<const S*>(a.b)[b * a.bb + nq * 4 + j] : 0.f;
-        Cv[j] = has ? (float)static_cast<const S*>(a.c)[b * a.cb + nq * 4 + j] : 0.f;
+    for (int j = 0; j < NS; ++j) {
+        const bool has = nq * NS + j < a.N;
+        Bv[j] = has ? (float)static_cast<const S*>(a.b)[b * a.bb + nq * NS + j] : 0.f;
+        Cv[j] = has ? (float)static_cast<const S*>(a.c)[b * a.cb + nq * NS + j] : 0.f;
     }
     const float u = (float)static_cast<const S*>(a.u)[b * a.ub + d];
     const float dt = step_of(a, (float)static_cast<const S*>(a.delta)[b * a.eb + d] + (a.dbias ? a.dbias[d] : 0.f));
     const float z = a.z ? (float)static_cast<const S*>(a.z)[b * a.zb + d] : 0.f;
     float y = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NS; ++j) {
         h[j] = fmaf(__builtin_amdgcn_exp2f(dt * (-LOG2E * rate_of(al[j]))), h[j], dt * u * Bv[j]);
         y = fmaf(Cv[j], h[j], y);
     }
     y = lanes_sum<LN>(y);
     if (!on) return;
-    store_states(a.h_out + s0, nq * 4, a.N, h);
+    store_states<NS>(a.h_out + s0, nq * NS, a.N, h);
     if (nq == 0) {
         y = fmaf(a.skip ? a.skip[d] : 0.f, u, y);
         static_cast<S*>(a.y)[(long long)b * a.D + d] = (S)(a.z ? y * (z * fast_sigmoid(z)) : y);
@@ -599,25 +795,27 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 
 // ------------------------------------------------------------------------------------------------ host
 struct ScanPlan {
-    int ln, np, cb, blocks, nrun, run;                   // blocks: channel blocks
+    int ln, ns, np, cb, blocks, nrun, run;               // blocks: channel blocks
     long long saved, ws;                                 // floats
     long long o_dt, o_bc, o_sums;                        // offsets in the workspace
 };
-// Frames are cut into runs where channel blocks x clips leave more than half of the CUs without a block: a cut costs the first launch
-// (about 0.9 of the main one's work), so the runs have to be at least four times as many blocks to pay.
+// Frames are cut into runs where channel blocks x clips leave CUs with hardly more than one block: a lone block per CU is bound by the
+// latency of its chain, and a cut costs the first launch (about 0.7 of the main one's work).  Measured: 192 blocks, T 1001, bf16: forward
+// 82 us uncut, 64 in 4 runs, 63 in 8, 89 in 16; backward 224, 155, 143, 168.  512 blocks, T 500, float: 50 uncut, 66 in 2; backward 146,
+// 163.  16 blocks, T 40000: 694 us in 8, 202 in 64, 188 in 256.
 static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     ScanPlan p{};
-    p.ln = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
-    p.np = 4 * p.ln;
+    p.ln = N <= 8 ? 4 : N <= 16 ? 8 : 16;
+    p.ns = N <= 32 ? 2 : 4;
+    p.np = p.ns * p.ln;
     p.cb = 256 / p.ln;
     p.blocks = (D + p.cb - 1) / p.cb;
-    const long long have = (long long)p.blocks * B, want = 2ll * device_cus();
+    const long long have = (long long)p.blocks * B, cus = device_cus();
     p.run = (T + 63) / 64 * 64;
-    if (have * 4 <= want) {
-        long long runs = (want + have - 1) / have;
-        if (runs > 64) runs = 64;
-        const int len = (int)(((T + runs - 1) / runs + 63) / 64 * 64);
-        if (len * 3 <= T) p.run = len;                   // at least three runs
+    if (have * 8 <= cus * 9) {
+        long long runs = (5 * cus + have - 1) / have;
+        if (runs > 256) runs = 256;
+        p.run = (int)(((T + runs - 1) / runs + 63) / 64 * 64);
     }
     p.nrun = (T + p.run - 1) / p.run;
     p.saved = (long long)((T + SC_SAVE - 1) / SC_SAVE) * B * D * p.np;
@@ -638,40 +836,47 @@ static int scan_check(const char* name, int T, int B, int D, int N, int dtype) {
     return PBSED_OK;
 }
 
-template <class S, int LN>
-static int scan_fwd_launch(const ScanArgs& a, const ScanPlan& p, hipStream_t s) {
+constexpr int SC_FOLD = 8;                               // up to so many runs the main launch folds those in front of its own by itself
+static int scan_fold(ScanArgs& a, const ScanPlan& p, int back, hipStream_t s) {
+    a.folded = p.nrun > SC_FOLD;
+    if (!a.folded) return PBSED_OK;
+    const long long blocks = ((long long)a.B * a.D * p.np + 63) / 64;
+    hipLaunchKernelGGL(scan_runs_kernel, dim3((unsigned)blocks), dim3(1024), 0, s, a, p.np, back);
+    return check_launch("selective_scan runs");
+}
+template <class S, int LN, int NS>
+static int scan_fwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
-        hipLaunchKernelGGL((scan_fwd_kernel<S, LN, true>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, true>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_fwd runs")) return rc;
+        if (const int rc = scan_fold(a, p, 0, s)) return rc;
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<S, LN, false>), dim3(p.blocks, a.B, p.nrun), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, false>), dim3(p.blocks, a.B, p.nrun), dim3(256), 0, s, a);
     return check_launch("selective_scan_fwd");
 }
-template <class S, int LN>
-static int scan_bwd_launch(const ScanArgs& a, const ScanPlan& p, hipStream_t s) {
+template <class S, int LN, int NS>
+static int scan_bwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
-        hipLaunchKernelGGL((scan_bwd_summary_kernel<S, LN>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((scan_bwd_summary_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_bwd runs")) return rc;
+        if (const int rc = scan_fold(a, p, 1, s)) return rc;
     }
-    constexpr size_t lds = (size_t)(3 * (256 / LN) * (SC_SAVE + 4) + 2 * SC_SAVE * 4 * LN + 4 * SC_SAVE * 8 * LN) * sizeof(float);
-    PBSED_DYN_LDS_ONCE((scan_bwd_kernel<S, LN>), lds);
-    hipLaunchKernelGGL((scan_bwd_kernel<S, LN>), dim3(p.blocks, a.B, p.nrun), dim3(256), lds, s, a);
+    constexpr size_t lds = ScanBwdLds<LN, NS>::bytes;
+    PBSED_DYN_LDS_ONCE((scan_bwd_kernel<S, LN, NS>), lds);
+    hipLaunchKernelGGL((scan_bwd_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun), dim3(256), lds, s, a);
     return check_launch("selective_scan_bwd");
 }
-template <class S, int LN>
-static int scan_step_launch(const ScanArgs& a, const ScanPlan& p, hipStream_t s) {
-    hipLaunchKernelGGL((scan_step_kernel<S, LN>), dim3(p.blocks, a.B), dim3(256), 0, s, a);
+template <class S, int LN, int NS>
+static int scan_step_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
+    hipLaunchKernelGGL((scan_step_kernel<S, LN, NS>), dim3(p.blocks, a.B), dim3(256), 0, s, a);
     return check_launch("selective_scan_step");
 }
 
-#define PBSED_SCAN(launch)                                      \
-    PBSED_ELEM(dtype, switch (p.ln) {                            \
-        case 1: rc = launch<S, 1>(a, p, s); break;               \
-        case 2: rc = launch<S, 2>(a, p, s); break;               \
-        case 4: rc = launch<S, 4>(a, p, s); break;               \
-        case 8: rc = launch<S, 8>(a, p, s); break;               \
-        default: rc = launch<S, 16>(a, p, s);                    \
-    })
+#define PBSED_SCAN(launch)                                                    \
+    PBSED_ELEM(dtype, rc = p.ln == 4 ? launch<S, 4, 2>(a, p, s)               \
+                           : p.ln == 8 ? launch<S, 8, 2>(a, p, s)             \
+                           : p.ns == 2 ? launch<S, 16, 2>(a, p, s)            \
+                                       : launch<S, 16, 4>(a, p, s))
 
 }  // namespace pbsed
 
@@ -685,6 +890,17 @@ extern "C" int pbsed_selective_scan_plan(int T, int B, int D, int N, int backwar
     return PBSED_OK;
 }
 
+// the tiles' 32-bit offsets reach over 64 frames
+static int scan_strides(const char* name, const long long* strides, int n, int B, int D) {
+    const long long most = (1ll << 31) / (64 * 4) - 1;
+    for (int i = 0; i < n; ++i)
+        if (strides[2 * i] < 0 || strides[2 * i] > most || strides[2 * i + 1] < 0 || (long long)B * D > most) {
+            set_error("%s: a frame stride of %lld elements (B * D = %lld); at most %lld", name, strides[2 * i], (long long)B * D, most);
+            return PBSED_E_UNSUPPORTED;
+        }
+    return PBSED_OK;
+}
+
 // strides (host): u, delta, b, c, z, each over frames and over clips
 extern "C" int pbsed_selective_scan_fwd(const void* u, const void* delta, const float* a_log, const void* b, const void* c, const float* skip,
                                         const void* z, const float* delta_bias, const int* seq_len, const float* state, void* y,
@@ -692,6 +908,7 @@ extern "C" int pbsed_selective_scan_fwd(const void* u, const void* delta, const 
                                         int T, int B, int D, int N, int softplus, int reverse, int dtype, void* stream) {
     if (const int rc = scan_check("selective_scan_fwd", T, B, D, N, dtype)) return rc;
     if (!u || !delta || !a_log || !b || !c || !y || !strides) { set_error("selective_scan_fwd: null pointer"); return PBSED_E_ARG; }
+    if (const int rc = scan_strides("selective_scan_fwd", strides, 5, B, D)) return rc;
     const ScanPlan p = scan_plan(T, B, D, N, false);
     if (p.ws && (!ws || ws_floats < p.ws || ((uintptr_t)ws & 15))) {
         set_error("selective_scan_fwd: needs a 16-byte aligned workspace of %lld floats, got %lld", p.ws, ws_floats);
@@ -723,6 +940,7 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
         set_error("selective_scan_bwd: null pointer");
         return PBSED_E_ARG;
     }
+    if (const int rc = scan_strides("selective_scan_bwd", strides, 7, B, D)) return rc;
     const ScanPlan p = scan_plan(T, B, D, N, true);
     if (!ws || ws_floats < p.ws || ((uintptr_t)ws & 15) || ((uintptr_t)saved & 15)) {
         set_error("selective_scan_bwd: needs a 16-byte aligned workspace of %lld floats (got %lld) and aligned saved states", p.ws, ws_floats);

@@ -299,6 +299,8 @@ template <class T> static inline void hipemu_buf_store(T v, __amdgpu_buffer_rsrc
 static inline hipemu_u32x4 __builtin_amdgcn_raw_buffer_load_b128(__amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { return hipemu_buf_load<hipemu_u32x4>(r, v, s); }
 static inline hipemu_u32x2 __builtin_amdgcn_raw_buffer_load_b64(__amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { return hipemu_buf_load<hipemu_u32x2>(r, v, s); }
 static inline unsigned __builtin_amdgcn_raw_buffer_load_b32(__amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { return hipemu_buf_load<unsigned>(r, v, s); }
+static inline unsigned short __builtin_amdgcn_raw_buffer_load_b16(__amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { return hipemu_buf_load<unsigned short>(r, v, s); }
+static inline void __builtin_amdgcn_raw_buffer_store_b16(unsigned short x, __amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { hipemu_buf_store(x, r, v, s); }
 static inline unsigned char __builtin_amdgcn_raw_buffer_load_b8(__amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { return hipemu_buf_load<unsigned char>(r, v, s); }
 static inline void __builtin_amdgcn_raw_buffer_store_b128(hipemu_u32x4 x, __amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { hipemu_buf_store(x, r, v, s); }
 static inline void __builtin_amdgcn_raw_buffer_store_b32(unsigned x, __amdgpu_buffer_rsrc_t r, unsigned v, unsigned s, int) { hipemu_buf_store(x, r, v, s); }
