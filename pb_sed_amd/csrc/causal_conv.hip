@@ -4,7 +4,8 @@
 // s runs over a clip's seq_len valid frames, forwards or (reverse) backwards; positions s < 0 hold `state` (zeros without one),
 // oldest first, and the state after the clip is its last K - 1 positions.  Frames behind a clip's end are not read; their outputs are 0.
 //
-// A thread owns V channels over a run of TS positions: the K-wide window slides through registers, so a tensor element is loaded once
+// A thread owns V channels (the last ones moved left until they end with D: the two threads that share channels there compute and
+// store the same values; addresses are those of any element, load_loose) over a run of TS positions: the K-wide window slides through registers, so a tensor element is loaded once
 // (plus K - 1 elements where two runs meet), in groups of G positions whose loads are all under way before the first is used.
 // Bound: HBM (x in, y out; backward x and dy in, dx out).
 #include "elem.h"
@@ -30,15 +31,17 @@ __device__ __forceinline__ void zero_v(float (&v)[V]) {
     for (int i = 0; i < V; ++i) v[i] = 0.f;
 }
 
-// grid (channel blocks, B * runs / RB): 64 channel vectors x RB runs per block of 256
+// forward: a wave = 64 channel vectors of a run, the channel groups of a run next to each other (a block reads whole rows); backward: grid
+// (channel groups, B * runs / RB), 64 channel vectors x RB runs per block of 256, whose sums for the weights meet in LDS
 constexpr int CC_RB = 4;
 
 template <class S, int V, int K>
 __global__ __launch_bounds__(256) void causal_conv_fwd_kernel(CConvArgs a) {
-    const int d0 = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
-    const long long unit = (long long)blockIdx.y * CC_RB + (threadIdx.x >> 6);
-    if (d0 >= a.D || unit >= (long long)a.B * a.nrun) return;
-    const int b = (int)(unit / a.nrun), run = (int)(unit % a.nrun);
+    const unsigned groups = (a.D + 64 * V - 1) / (64 * V), wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int dv = ((int)(wave % groups) * 64 + (int)(threadIdx.x & 63)) * V, d0 = min(dv, a.D - V);
+    const int unit = wave / groups;
+    if (dv >= a.D || unit >= a.B * a.nrun) return;
+    const int b = unit / a.nrun, run = unit % a.nrun;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
     const int p0 = run * a.ts, p1 = min(p0 + a.ts, a.T);
     const S* x = static_cast<const S*>(a.x) + b * a.xb + d0;
@@ -55,16 +58,16 @@ __global__ __launch_bounds__(256) void causal_conv_fwd_kernel(CConvArgs a) {
     for (int j = 0; j < K - 1; ++j) {
         const int p = p0 - (K - 1) + j;
         if (p >= 0) {
-            if (p < len) load_pack<S, V>(x + frame(p) * a.xt, win[j]);
+            if (p < len) load_loose<S, V>(x + frame(p) * a.xt, win[j]);
             else zero_v<S, V>(win[j]);
-        } else if (a.state) load_pack<S, V>(static_cast<const S*>(a.state) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, win[j]);
+        } else if (a.state) load_loose<S, V>(static_cast<const S*>(a.state) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, win[j]);
         else zero_v<S, V>(win[j]);
     }
     // (a valid position's window holds valid positions and the state only: what zero_v stands for behind the end is never used)
     auto keep = [&](int end) {                  // the window in front of position `end` = len is the state behind the clip
         if (a.state_out && end == len)
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) store_pack<S, V>(static_cast<S*>(a.state_out) + ((long long)b * (K - 1) + j) * a.D + d0, win[j]);
+            for (int j = 0; j < K - 1; ++j) store_loose<S, V>(static_cast<S*>(a.state_out) + ((long long)b * (K - 1) + j) * a.D + d0, win[j]);
     };
     if (run == 0) keep(0);
     auto one = [&](int p, const float (&cur)[V]) __attribute__((always_inline)) {
@@ -77,7 +80,7 @@ __global__ __launch_bounds__(256) void causal_conv_fwd_kernel(CConvArgs a) {
             s = fmaf(w[K - 1][v], cur[v], s);
             o[v] = a.silu ? s * fast_sigmoid(s) : s;
         }
-        store_pack<S, V>(y + frame(p) * a.yt, o);
+        store_loose<S, V>(y + frame(p) * a.yt, o);
 #pragma unroll
         for (int j = 0; j + 1 < K - 1; ++j)
 #pragma unroll
@@ -90,28 +93,28 @@ __global__ __launch_bounds__(256) void causal_conv_fwd_kernel(CConvArgs a) {
     for (; p + CC_G <= valid; p += CC_G) {
         float cur[CC_G][V];
 #pragma unroll
-        for (int i = 0; i < CC_G; ++i) load_pack<S, V>(x + frame(p + i) * a.xt, cur[i]);
+        for (int i = 0; i < CC_G; ++i) load_loose<S, V>(x + frame(p + i) * a.xt, cur[i]);
 #pragma unroll
         for (int i = 0; i < CC_G; ++i) one(p + i, cur[i]);
     }
     for (; p < valid; ++p) {
         float cur[V];
-        load_pack<S, V>(x + frame(p) * a.xt, cur);
+        load_loose<S, V>(x + frame(p) * a.xt, cur);
         one(p, cur);
     }
     if (p > p0 && p == len) keep(p);
     float z[V];
     zero_v<S, V>(z);
-    for (p = max(p, p0); p < p1; ++p) store_pack<S, V>(y + (long long)p * a.yt, z);
+    for (p = max(p, p0); p < p1; ++p) store_loose<S, V>(y + (long long)p * a.yt, z);
 }
 
 template <class S, int V, int K>
 __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
     __shared__ float red[CC_RB][64][V * (K + 1) + 1];
     const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
-    const int d0 = (blockIdx.x * 64 + lane) * V;
+    const int dv = (blockIdx.x * 64 + lane) * V, d0 = min(dv, a.D - V);
     const long long unit = (long long)blockIdx.y * CC_RB + sub;
-    const bool on = d0 < a.D && unit < (long long)a.B * a.nrun;
+    const bool on = dv < a.D && unit < (long long)a.B * a.nrun;
     float dw[K][V], db[V];
     zero_v<S, V>(db);
 #pragma unroll
@@ -133,21 +136,21 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
         }
         auto input = [&](int p, float (&o)[V]) {
             if (p >= 0) {
-                if (p < len) load_pack<S, V>(x + frame(p) * a.xt, o);
+                if (p < len) load_loose<S, V>(x + frame(p) * a.xt, o);
                 else zero_v<S, V>(o);
-            } else if (a.state) load_pack<S, V>(static_cast<const S*>(a.state) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, o);
+            } else if (a.state) load_loose<S, V>(static_cast<const S*>(a.state) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, o);
             else zero_v<S, V>(o);
         };
         auto emit = [&](int p, float (&o)[V]) {                     // gradient of position p (p < 0: of the state); the state behind
             const int k = p - (len - (K - 1));                      // the clip is its last K - 1 positions: their gradients meet here
             if (a.dstate_out && k >= 0 && k < K - 1) {
                 float e[V];
-                load_pack<S, V>(static_cast<const S*>(a.dstate_out) + ((long long)b * (K - 1) + k) * a.D + d0, e);
+                load_loose<S, V>(static_cast<const S*>(a.dstate_out) + ((long long)b * (K - 1) + k) * a.D + d0, e);
 #pragma unroll
                 for (int v = 0; v < V; ++v) o[v] += e[v];
             }
-            if (p >= 0) store_pack<S, V>(dx + frame(p) * a.yt, o);
-            else if (a.state_out) store_pack<S, V>(static_cast<S*>(a.state_out) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, o);
+            if (p >= 0) store_loose<S, V>(dx + frame(p) * a.yt, o);
+            else if (a.state_out) store_loose<S, V>(static_cast<S*>(a.state_out) + ((long long)b * (K - 1) + K - 1 + p) * a.D + d0, o);
         };
         // run 0 also owns the K - 1 positions of the state: its gradients come out while the window fills
         const int first = run == 0 && a.state_out ? -(K - 1) : p0;
@@ -192,8 +195,8 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
                 float cur[CC_G][V], g[CC_G][V];
 #pragma unroll
                 for (int i = 0; i < CC_G; ++i) {
-                    load_pack<S, V>(x + frame(q + i) * a.xt, cur[i]);
-                    load_pack<S, V>(dy + frame(q + i) * a.gt, g[i]);
+                    load_loose<S, V>(x + frame(q + i) * a.xt, cur[i]);
+                    load_loose<S, V>(dy + frame(q + i) * a.gt, g[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < CC_G; ++i) one(q + i, cur[i], g[i], true);
@@ -203,14 +206,14 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
             for (; q < stop; ++q) {
                 float cur[V], g[V];
                 input(q, cur);
-                if (q < len) load_pack<S, V>(dy + frame(q) * a.gt, g);
+                if (q < len) load_loose<S, V>(dy + frame(q) * a.gt, g);
                 else zero_v<S, V>(g);
                 one(q, cur, g, q < valid);
             }
         }
         float z[V];
         zero_v<S, V>(z);
-        for (int p = max(valid, p0); p < p1; ++p) store_pack<S, V>(dx + (long long)p * a.yt, z);
+        for (int p = max(valid, p0); p < p1; ++p) store_loose<S, V>(dx + (long long)p * a.yt, z);
     }
     if (!a.ws) return;
 #pragma unroll
@@ -223,15 +226,16 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
     // partial row: dw [D][K], then db [D]
     float* out = a.ws + (long long)blockIdx.y * a.D * (K + 1);
     for (int i = threadIdx.x; i < 64 * V * (K + 1); i += 256) {
-        const int l = i / (V * (K + 1)), e = i % (V * (K + 1)), d = (blockIdx.x * 64 + l) * V + e / (K + 1), j = e % (K + 1);
-        if (d >= a.D) continue;
+        const int l = i / (V * (K + 1)), e = i % (V * (K + 1)), first = (blockIdx.x * 64 + l) * V, j = e % (K + 1);
+        if (first >= a.D) continue;
+        const int d = min(first, a.D - V) + e / (K + 1);
         const float s = (red[0][l][e] + red[1][l][e]) + (red[2][l][e] + red[3][l][e]);
         out[j < K ? (long long)d * K + j : (long long)a.D * K + d] = s;
     }
 }
 
-__global__ __launch_bounds__(256) void causal_conv_sum_kernel(const float* ws, int P, long W, SumSegs sg) {
-    __shared__ double red[16 * 17];
+__global__ __launch_bounds__(SUM_THREADS) void causal_conv_sum_kernel(const float* ws, int P, long W, SumSegs sg) {
+    __shared__ double red[SUM_LDS];
     sum_partials(ws, P, W, sg, blockIdx.x * 16, red);
 }
 
@@ -264,20 +268,13 @@ static int cconv_ts(int T, int B, int D, int V) {
     while ((long long)B * ((T + ts - 1) / ts) > 65535ll * CC_RB && ts < (1 << 29)) ts <<= 1;      // the grid's second dimension
     return ts;
 }
-static int cconv_v(const CConvArgs& a, int esize, bool bwd) {
-    const int full = bwd ? 4 : 16 / esize;
-    const long long odd = a.D | a.xt | a.xb | a.yt | a.yb | (bwd ? a.gt | a.gb : 0);
-    const uintptr_t p = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.state | (uintptr_t)a.state_out | (uintptr_t)a.dstate_out;
-    return !(odd % full) && !(p % (full * esize)) ? full : 1;
-}
-
 template <class S, int V, int K>
 static void cconv_launch3(const CConvArgs& a, bool bwd, hipStream_t s) {
     const long long units = (long long)a.B * a.nrun;
     const dim3 grid((a.D + 64 * V - 1) / (64 * V), (unsigned)((units + CC_RB - 1) / CC_RB));
     if (bwd) {
         if constexpr (V <= 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<S, V, K>), grid, dim3(256), 0, s, a);
-    } else hipLaunchKernelGGL((causal_conv_fwd_kernel<S, V, K>), grid, dim3(256), 0, s, a);
+    } else hipLaunchKernelGGL((causal_conv_fwd_kernel<S, V, K>), dim3((unsigned)((units * grid.x + 3) / 4)), dim3(256), 0, s, a);
 }
 template <class S, int V>
 static void cconv_launch2(const CConvArgs& a, int K, bool bwd, hipStream_t s) {
@@ -293,7 +290,7 @@ static void cconv_launch2(const CConvArgs& a, int K, bool bwd, hipStream_t s) {
 }
 template <class S>
 static int cconv_launch(CConvArgs& a, int K, bool bwd, hipStream_t s) {
-    const int v = cconv_v(a, sizeof(S), bwd);
+    const int full = bwd ? 4 : 16 / (int)sizeof(S), v = a.D >= full ? full : 1;
     a.ts = cconv_ts(a.T, a.B, a.D, v);
     a.nrun = (a.T + a.ts - 1) / a.ts;
     if (v == 1) cconv_launch2<S, 1>(a, K, bwd, s);
@@ -365,7 +362,7 @@ extern "C" int pbsed_causal_conv_bwd(const void* dy, const void* x, const float*
     const long W = (long)D * (K + 1);
     const SumSegs sg{{dw, db, nullptr}, {D * K, D * (K + 1), D * (K + 1)}};
     const int P = (int)(((long long)B * a.nrun + CC_RB - 1) / CC_RB);
-    hipLaunchKernelGGL(causal_conv_sum_kernel, dim3((unsigned)((W + 15) / 16)), dim3(256), 0, (hipStream_t)stream, ws, P, W, sg);
+    hipLaunchKernelGGL(causal_conv_sum_kernel, dim3((unsigned)((W + 15) / 16)), dim3(SUM_THREADS), 0, (hipStream_t)stream, ws, P, W, sg);
     return check_launch("causal_conv_bwd sums");
 }
 

@@ -42,6 +42,8 @@ __device__ __forceinline__ void philox7(unsigned long long block, unsigned step,
     w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
 }
 
+__device__ __forceinline__ float dropped(const DropoutArgs& a, unsigned word, float v) { return word >= a.thr && !a.drop_all ? v * a.scale : 0.f; }
+
 // V elements per thread and turn.  FLAT: one run of n elements.  Otherwise rows of C (a multiple of V) at their strides.
 template <class S, int V, bool FLAT>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
@@ -60,8 +62,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
         float v[V], w[V];
         const bool whole = i0 + V <= a.n;
         if (whole) {
-            load_pack<S, V>(x, v);
-            if (a.res) load_pack<S, V>(res, w);
+            load_loose<S, V>(x, v);
+            if (a.res) load_loose<S, V>(res, w);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -73,11 +75,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if (j % 4 == 0) philox7((unsigned long long)(i0 + j) >> 2, step, a.site, k0, k1, bits);
-            const unsigned word = V >= 4 ? bits[j & 3] : ((i0 & 3) == 0 ? bits[0] : (i0 & 3) == 1 ? bits[1] : (i0 & 3) == 2 ? bits[2] : bits[3]);
-            v[j] = word >= a.thr && !a.drop_all ? v[j] * a.scale : 0.f;
+            v[j] = dropped(a, bits[j & 3], v[j]);
             if (a.res) v[j] += w[j];
         }
-        if (whole) store_pack<S, V>(y, v);
+        if (whole) store_loose<S, V>(y, v);
         else
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -85,23 +86,39 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
     }
 }
 
-template <class S, int V, bool FLAT>
-static int dropout_launch(const DropoutArgs& a, hipStream_t s) {
-    const long long blocks = ((a.n + V - 1) / V + 255) / 256;
-    // one turn per thread up to 16 blocks per CU, then a loop
-    const long long most = (long long)device_cus() * 16;
-    hipLaunchKernelGGL((dropout_kernel<S, V, FLAT>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, a);
-    return check_launch("dropout");
+// rows of any width at any strides: the generator's groups of four run on across row ends
+template <class S>
+__global__ __launch_bounds__(256) void dropout_rows_kernel(DropoutArgs a) {
+    const unsigned k0 = (unsigned)a.rng[0], k1 = (unsigned)((unsigned long long)a.rng[0] >> 32), step = (unsigned)a.rng[1];
+    const long long groups = (a.n + 3) / 4, stride = (long long)gridDim.x * 256;
+    for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < groups; g += stride) {
+        const long long i0 = g * 4;
+        long long r = a.n <= 0x7fffffffll ? (long long)((unsigned)i0 / a.C) : i0 / a.C;
+        unsigned c = (unsigned)(i0 - r * a.C), bits[4];
+        philox7((unsigned long long)g, step, a.site, k0, k1, bits);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i0 + j >= a.n) break;
+            float v = dropped(a, bits[j], (float)static_cast<const S*>(a.x)[r * a.xs + c]);
+            if (a.res) v += (float)static_cast<const S*>(a.res)[r * a.rs + c];
+            static_cast<S*>(a.y)[r * a.ys + c] = (S)v;
+            if (++c == a.C) { c = 0; ++r; }
+        }
+    }
 }
 
 template <class S>
-static int dropout_dispatch(const DropoutArgs& a, hipStream_t s) {
+static int dropout_launch(const DropoutArgs& a, hipStream_t s) {
     constexpr int V = 16 / sizeof(S);
-    const bool flat = a.xs == a.C && a.ys == a.C && (!a.res || a.rs == a.C);
-    const bool aligned = !(((uintptr_t)a.x | (uintptr_t)a.res | (uintptr_t)a.y) & 15);
-    if (aligned && flat) return dropout_launch<S, V, true>(a, s);
-    if (aligned && !((a.C | a.xs | a.ys | (a.res ? a.rs : 0)) % V)) return dropout_launch<S, V, false>(a, s);
-    return dropout_launch<S, 1, false>(a, s);
+    const bool flat = a.xs == a.C && a.ys == a.C && (!a.res || a.rs == a.C), vec = flat || a.C % V == 0;
+    const long long per = vec ? V : 4, blocks = ((a.n + per - 1) / per + 255) / 256;
+    // one turn per thread up to 16 blocks per CU, then a loop
+    const long long most = (long long)device_cus() * 16;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    if (flat) hipLaunchKernelGGL((dropout_kernel<S, V, true>), grid, dim3(256), 0, s, a);
+    else if (vec) hipLaunchKernelGGL((dropout_kernel<S, V, false>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(dropout_rows_kernel<S>, grid, dim3(256), 0, s, a);
+    return check_launch("dropout");
 }
 
 }  // namespace pbsed
@@ -126,5 +143,5 @@ extern "C" int pbsed_dropout(const void* x, const void* residual, void* y, long 
     a.drop_all = p >= 1.;
     a.thr = a.drop_all ? 0xffffffffu : (unsigned)(p * 4294967296.);
     a.scale = a.drop_all ? 0.f : (float)(1. / (1. - p));
-    PBSED_ELEM(dtype, return dropout_dispatch<S>(a, (hipStream_t)stream));
+    PBSED_ELEM(dtype, return dropout_launch<S>(a, (hipStream_t)stream));
 }

@@ -8,6 +8,8 @@ namespace pbsed {
 enum { PBSED_DT_F32 = 0, PBSED_DT_BF16 = 1, PBSED_DT_F16 = 2 };
 
 template <class S, int V> struct alignas(sizeof(S) * V) Pack { S v[V]; };
+// the same at any address of an S: gfx950 reads and writes up to 16 bytes of global memory at any 2-byte address in one instruction
+template <class S, int V> struct __attribute__((packed, aligned(sizeof(S)))) LoosePack { S v[V]; };
 
 template <class S, int V>
 __device__ __forceinline__ void load_pack(const S* p, float (&out)[V]) {
@@ -21,6 +23,20 @@ __device__ __forceinline__ void store_pack(S* p, const float (&in)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) w.v[i] = (S)in[i];
     *reinterpret_cast<Pack<S, V>*>(p) = w;
+}
+
+template <class S, int V>
+__device__ __forceinline__ void load_loose(const S* p, float (&out)[V]) {
+    const LoosePack<S, V> w = *reinterpret_cast<const LoosePack<S, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)w.v[i];
+}
+template <class S, int V>
+__device__ __forceinline__ void store_loose(S* p, const float (&in)[V]) {
+    LoosePack<S, V> w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w.v[i] = (S)in[i];
+    *reinterpret_cast<LoosePack<S, V>*>(p) = w;
 }
 
 __device__ __forceinline__ float fast_sigmoid(float x) {           // v_exp_f32 + v_rcp_f32: 1 ulp each
@@ -50,18 +66,35 @@ __device__ __forceinline__ float softplus(float x) {
 // out[i] += sum over p < P of ws[p][i]: the last step of a reduction whose blocks have left one row of partial sums each, in a fixed
 // order (results do not depend on the order in which the blocks ran); partials are added in double.  A segment = one output.
 struct SumSegs { float* out[3]; int end[3]; };                      // out may be null; end: first index behind the segment
-// grid ceil(W / 16), 256 threads: 16 columns x 16 groups of rows
+// grid ceil(W / 16), 1024 threads: 16 columns x 64 groups of rows
+constexpr int SUM_THREADS = 1024, SUM_LDS = 64 * 17;
 __device__ __forceinline__ void sum_partials(const float* ws, int P, long W, const SumSegs& sg, int col0, double* red) {
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
     const long col = col0 + c;
     double acc = 0.;
-    if (col < W)
-        for (int p = g; p < P; p += 16) acc += (double)ws[(long)p * W + col];
+    if (col < W) {
+        const float* p = ws + g * W + col;
+        const long step = 64 * W;
+        int n = g < P ? (P - g + 63) / 64 : 0;
+        for (; n >= 8; n -= 8, p += 8 * step) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = p[k * step];
+            acc += (((double)v[0] + v[1]) + ((double)v[2] + v[3])) + (((double)v[4] + v[5]) + ((double)v[6] + v[7]));
+        }
+        for (; n > 0; --n, p += step) acc += (double)*p;
+    }
     red[g * 17 + c] = acc;
+    __syncthreads();
+    if (g < 8) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) acc += red[(g + 8 * k) * 17 + c];
+        red[g * 17 + c] = acc;
+    }
     __syncthreads();
     if (g == 0 && col < W) {
 #pragma unroll
-        for (int k = 1; k < 16; ++k) acc += red[k * 17 + c];
+        for (int k = 1; k < 8; ++k) acc += red[k * 17 + c];
         int s = 0;
         while (s < 2 && col >= sg.end[s]) ++s;
         float* o = sg.out[s];

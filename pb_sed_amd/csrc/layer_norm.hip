@@ -40,125 +40,147 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
-// columns of a lane: (k LPR + lane) V + j, k < E / V, j < V
-template <class S, int V, int LPR, int E>
-__device__ __forceinline__ void load_row(const S* row, int lane, int C, float (&v)[E]) {
+// A lane's columns: E / V vectors of V, vector k from (k LPR + lane) V on.  Where C is no multiple of V (TAIL), the last vector of a row is
+// moved left until it ends with the row: its first columns are the neighbour's too, both lanes compute and store the same values, and
+// `m` (0 there, 1 elsewhere) keeps them out of the row's sums.  Rows start at any element (load_loose).
+template <int V, int LPR, int E, bool TAIL> struct NormCols {
+    int c[E / V];                                                   // first column, -1: none
+    float m[TAIL ? E : 1];
+    __device__ __forceinline__ NormCols(int lane, int C) {
 #pragma unroll
-    for (int k = 0; k < E / V; ++k) {
-        const int c = (k * LPR + lane) * V;
-        float p[V];
-        if (c < C) load_pack<S, V>(row + c, p);
-        else
+        for (int k = 0; k < E / V; ++k) {
+            const int c0 = (k * LPR + lane) * V;
+            c[k] = c0 >= C ? -1 : TAIL && c0 + V > C ? C - V : c0;
+            if constexpr (TAIL)
 #pragma unroll
-            for (int j = 0; j < V; ++j) p[j] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[k * V + j] = p[j];
-    }
-}
-template <class S, int V, int LPR, int E>
-__device__ __forceinline__ void store_row(S* row, int lane, int C, const float (&v)[E]) {
-#pragma unroll
-    for (int k = 0; k < E / V; ++k) {
-        const int c = (k * LPR + lane) * V;
-        float p[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = v[k * V + j];
-        if (c < C) store_pack<S, V>(row + c, p);
-    }
-}
-// weights: float, same columns; their rows are 4-byte aligned only
-template <int V, int LPR, int E>
-__device__ __forceinline__ void load_weights(const float* w, float none, int lane, int C, float (&v)[E]) {
-#pragma unroll
-    for (int k = 0; k < E / V; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (k * LPR + lane) * V + j;
-            v[k * V + j] = w && c < C ? w[c] : none;
+                for (int j = 0; j < V; ++j) m[k * V + j] = c0 < C && c[k] + j >= c0 ? 1.f : 0.f;
         }
-}
+    }
+    __device__ __forceinline__ float own(int e) const {            // (without TAIL every column that a lane has is its own)
+        if constexpr (TAIL) return m[e];
+        return 1.f;
+    }
+    // a row on its way (in its own type: half the registers of its values for 16-bit elements), and its values
+    template <class S> struct Raw { LoosePack<S, V> p[E / V]; };
+    template <class S> __device__ __forceinline__ void fetch(const S* row, Raw<S>& raw) const {
+#pragma unroll
+        for (int k = 0; k < E / V; ++k)
+            if (c[k] >= 0) raw.p[k] = *reinterpret_cast<const LoosePack<S, V>*>(row + c[k]);
+    }
+    template <class S> __device__ __forceinline__ void values(const Raw<S>& raw, bool on, float (&v)[E]) const {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = on && c[e / V] >= 0 ? (float)raw.p[e / V].v[e % V] : 0.f;
+    }
+    template <class S> __device__ __forceinline__ void store(S* row, const float (&v)[E]) const {
+#pragma unroll
+        for (int k = 0; k < E / V; ++k) {
+            float p[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) p[j] = v[k * V + j];
+            if (c[k] >= 0) store_loose<S, V>(row + c[k], p);
+        }
+    }
+    __device__ __forceinline__ void weights(const float* w, float none, float (&v)[E]) const {
+        constexpr int W = V < 4 ? V : 4;
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+            float p[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) p[j] = none;
+            if (w && c[i * W / V] >= 0) load_loose<float, W>(w + c[i * W / V] + i * W % V, p);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i * W + j] = p[j];
+        }
+    }
+};
 
-template <class S, int V, int LPR, int E>
+template <class S, int V, int LPR, int E, bool TAIL>
 __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(NormArgs a) {
     __shared__ float red[4];
     constexpr int RPB = 256 / LPR;                                  // rows of a block side by side
     const int lane = threadIdx.x % LPR;
-    float w[E], b[E];
-    load_weights<V, LPR, E>(a.w, 1.f, lane, a.C, w);
-    load_weights<V, LPR, E>(a.b, 0.f, lane, a.C, b);
-    const float inv = 1.f / (float)a.C;
+    const NormCols<V, LPR, E, TAIL> cols(lane, a.C);
+    float w[E], b[E], v[E];
+    typename NormCols<V, LPR, E, TAIL>::template Raw<S> raw;
     const int step = gridDim.x * RPB;
     int r = blockIdx.x * RPB + threadIdx.x / LPR;
-    float v[E];
-    if (r < a.rows) load_row<S, V, LPR, E>(static_cast<const S*>(a.x) + r * a.xs, lane, a.C, v);
+    const S* x = static_cast<const S*>(a.x);
+    if (r < a.rows) cols.fetch(x + r * a.xs, raw);
+    cols.weights(a.w, 1.f, w);
+    cols.weights(a.b, 0.f, b);
+    const float inv = 1.f / (float)a.C;
     // (every lane of a block makes the same number of turns: row_sum has barriers where LPR is the block)
     for (int r0 = blockIdx.x * RPB; r0 < a.rows; r0 += step, r += step) {
-        float nxt[E];
-        if (r + step < a.rows) load_row<S, V, LPR, E>(static_cast<const S*>(a.x) + (long long)(r + step) * a.xs, lane, a.C, nxt);
+        cols.values(raw, true, v);
+        if (r + step < a.rows) cols.fetch(x + (long long)(r + step) * a.xs, raw);
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += v[e];
+        for (int e = 0; e < E; ++e) s = fmaf(v[e], cols.own(e), s);
         const float mean = row_sum<LPR>(s, red) * inv;
         s = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            v[e] = (e / V * LPR + lane) * V + e % V < a.C ? v[e] - mean : 0.f;
-            s = fmaf(v[e], v[e], s);
+            v[e] = cols.c[e / V] >= 0 ? v[e] - mean : 0.f;
+            s = fmaf(v[e] * cols.own(e), v[e], s);
         }
         const float rstd = 1.f / sqrtf(fmaf(row_sum<LPR>(s, red), inv, a.eps));
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = fmaf(v[e] * rstd, w[e], b[e]);
         if (r < a.rows) {
-            store_row<S, V, LPR, E>(static_cast<S*>(a.y) + (long long)r * a.C, lane, a.C, v);
+            cols.store(static_cast<S*>(a.y) + (long long)r * a.C, v);
             if (a.stats && lane == 0) *reinterpret_cast<float2*>(a.stats + 2ll * r) = make_float2(mean, rstd);
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = nxt[e];
     }
 }
 
-template <class S, int V, int LPR, int E>
+template <class S, int V, int LPR, int E, bool TAIL>
 __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(NormArgs a) {
     __shared__ float red[4];
     constexpr int RPB = 256 / LPR;
-    __shared__ float cols[RPB > 1 ? RPB * LPR * 2 * V : 1];         // one column chunk of the rows' sums at a time
+    __shared__ float part[RPB > 1 ? RPB * LPR * 2 * V : 1];         // one vector per lane of the rows' sums at a time
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const NormCols<V, LPR, E, TAIL> cols(lane, a.C);
     float w[E], dw[E], db[E];
-    load_weights<V, LPR, E>(a.w, 1.f, lane, a.C, w);
+    cols.weights(a.w, 1.f, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
     const float inv = 1.f / (float)a.C;
     const int step = gridDim.x * RPB;
     int r = blockIdx.x * RPB + sub;
+    typename NormCols<V, LPR, E, TAIL>::template Raw<S> rx, rg;
+    float2 rst = make_float2(0.f, 0.f);
+    auto fetch = [&](int q) __attribute__((always_inline)) {
+        if (q >= a.rows) return;
+        cols.fetch(static_cast<const S*>(a.x) + q * a.xs, rx);
+        cols.fetch(static_cast<const S*>(a.dy) + q * a.dys, rg);
+        rst = *reinterpret_cast<const float2*>(a.stats + 2ll * q);
+    };
+    fetch(r);
     for (int r0 = blockIdx.x * RPB; r0 < a.rows; r0 += step, r += step) {
         const bool on = r < a.rows;
         float x[E], dy[E];
-        float2 st = make_float2(0.f, 0.f);
-        if (on) {
-            load_row<S, V, LPR, E>(static_cast<const S*>(a.x) + r * a.xs, lane, a.C, x);
-            load_row<S, V, LPR, E>(static_cast<const S*>(a.dy) + r * a.dys, lane, a.C, dy);
-            st = *reinterpret_cast<const float2*>(a.stats + 2ll * r);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = dy[e] = 0.f;
-        }
+        const float2 st = rst;
+        cols.values(rx, on, x);
+        cols.values(rg, on, dy);
+        fetch(r + step);
         float sg = 0.f, sgx = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {                               // behind the row's end dy = 0: nothing is added
+        for (int e = 0; e < E; ++e) {                               // where a lane has no column dy = 0: nothing is added
             x[e] = (x[e] - st.x) * st.y;
             dw[e] = fmaf(dy[e], x[e], dw[e]);
             db[e] += dy[e];
             dy[e] *= w[e];
-            sg += dy[e];
-            sgx = fmaf(dy[e], x[e], sgx);
+            const float g = dy[e] * cols.own(e);
+            sg += g;
+            sgx = fmaf(g, x[e], sgx);
         }
         const float mg = row_sum<LPR>(sg, red) * inv, mgx = row_sum<LPR>(sgx, red) * inv;
 #pragma unroll
         for (int e = 0; e < E; ++e) dy[e] = st.y * (dy[e] - mg - x[e] * mgx);
-        if (on) store_row<S, V, LPR, E>(static_cast<S*>(a.y) + (long long)r * a.C, lane, a.C, dy);
+        if (on) cols.store(static_cast<S*>(a.y) + (long long)r * a.C, dy);
     }
     if (!a.ws) return;
-    // the RPB rows side by side meet in LDS, chunk after chunk; lanes of sub 0 write the block's partials
+    // the RPB rows side by side meet in LDS, vector after vector; lanes of sub 0 write the block's partials
     float* out = a.ws + (long long)blockIdx.x * 2 * a.C;
 #pragma unroll
     for (int k = 0; k < E / V; ++k) {
@@ -166,22 +188,23 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(NormArgs a) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                cols[((sub * V + j) * 2) * LPR + lane] = dw[k * V + j];
-                cols[((sub * V + j) * 2 + 1) * LPR + lane] = db[k * V + j];
+                part[((sub * V + j) * 2) * LPR + lane] = dw[k * V + j];
+                part[((sub * V + j) * 2 + 1) * LPR + lane] = db[k * V + j];
             }
             __syncthreads();
         }
-        if (sub == 0)
+        if (sub == 0 && cols.c[k] >= 0)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 float s0 = dw[k * V + j], s1 = db[k * V + j];
 #pragma unroll
                 for (int q = 1; q < RPB; ++q) {
-                    s0 += cols[((q * V + j) * 2) * LPR + lane];
-                    s1 += cols[((q * V + j) * 2 + 1) * LPR + lane];
+                    s0 += part[((q * V + j) * 2) * LPR + lane];
+                    s1 += part[((q * V + j) * 2 + 1) * LPR + lane];
                 }
-                const int c = (k * LPR + lane) * V + j;
-                if (c < a.C) { out[c] = s0; out[a.C + c] = s1; }
+                // (a column that two lanes have: both hold the same sums)
+                out[cols.c[k] + j] = s0;
+                out[a.C + cols.c[k] + j] = s1;
             }
     }
 }
@@ -231,8 +254,8 @@ __global__ __launch_bounds__(256) void layer_norm_wide_bwd_kernel(NormArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void norm_sum_kernel(const float* ws, int P, long W, SumSegs sg) {
-    __shared__ double red[16 * 17];
+__global__ __launch_bounds__(SUM_THREADS) void norm_sum_kernel(const float* ws, int P, long W, SumSegs sg) {
+    __shared__ double red[SUM_LDS];
     sum_partials(ws, P, W, sg, blockIdx.x * 16, red);
 }
 
@@ -243,17 +266,23 @@ static void norm_shape(int C, int* lpr, int* e) {
     else if (C <= 2048) { *lpr = 64; *e = 32; }
     else { *lpr = 256; *e = C <= 4096 ? 16 : 32; }
 }
+// blocks that a CU holds at once: every one walks its rows without a second wave of blocks behind it, and the partial sums stay few
 static int norm_grid(int rows, int C, bool bwd) {
-    int lpr = 256, e;
+    int lpr = 256, e = 32;
     if (C <= 8192) norm_shape(C, &lpr, &e);
-    const int rpb = 256 / lpr, need = (rows + rpb - 1) / rpb, most = device_cus() * (bwd ? 4 : 8);
+    const int rpb = 256 / lpr, need = (rows + rpb - 1) / rpb, most = device_cus() * (bwd ? (e >= 32 ? 1 : e == 16 ? 2 : 4) : (e >= 32 ? 2 : e == 16 ? 4 : 8));
     return need < most ? need : most;
 }
 
 template <class S, int V, int LPR, int E>
 static void norm_launch2(const NormArgs& a, bool bwd, int grid, hipStream_t s) {
-    if (bwd) hipLaunchKernelGGL((layer_norm_bwd_kernel<S, V, LPR, E>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((layer_norm_fwd_kernel<S, V, LPR, E>), dim3(grid), dim3(256), 0, s, a);
+    if (a.C % V) {
+        if (bwd) hipLaunchKernelGGL((layer_norm_bwd_kernel<S, V, LPR, E, true>), dim3(grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((layer_norm_fwd_kernel<S, V, LPR, E, true>), dim3(grid), dim3(256), 0, s, a);
+    } else {
+        if (bwd) hipLaunchKernelGGL((layer_norm_bwd_kernel<S, V, LPR, E, false>), dim3(grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((layer_norm_fwd_kernel<S, V, LPR, E, false>), dim3(grid), dim3(256), 0, s, a);
+    }
 }
 template <class S, int V>
 static void norm_launch1(const NormArgs& a, bool bwd, int grid, hipStream_t s) {
@@ -275,12 +304,9 @@ static int norm_launch(const NormArgs& a, bool bwd, hipStream_t s) {
     if (a.C > 8192) {
         if (bwd) hipLaunchKernelGGL(layer_norm_wide_bwd_kernel<S>, dim3(grid), dim3(256), 0, s, a);
         else hipLaunchKernelGGL(layer_norm_wide_fwd_kernel<S>, dim3(grid), dim3(256), 0, s, a);
-    } else {
-        const long long odd = a.C | a.xs | (bwd ? a.dys : 0);
-        const bool vec = !(odd % V) && !(((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.dy) & 15);
-        if (vec) norm_launch1<S, V>(a, bwd, grid, s);
-        else norm_launch1<S, 1>(a, bwd, grid, s);
-    }
+    } else if (a.C >= V) norm_launch1<S, V>(a, bwd, grid, s);
+    else if (bwd) hipLaunchKernelGGL((layer_norm_bwd_kernel<S, 1, 16, 4, false>), dim3(grid), dim3(256), 0, s, a);      // rows shorter than a vector
+    else hipLaunchKernelGGL((layer_norm_fwd_kernel<S, 1, 16, 4, false>), dim3(grid), dim3(256), 0, s, a);
     return check_launch(bwd ? "layer_norm_bwd" : "layer_norm_fwd");
 }
 
@@ -329,6 +355,6 @@ extern "C" int pbsed_layer_norm_bwd(const void* dy, const void* x, const float* 
     PBSED_ELEM(dtype, rc = norm_launch<S>(a, true, (hipStream_t)stream));
     if (rc || !sums) return rc;
     const SumSegs sg{{dw, db, nullptr}, {(int)C, (int)(2 * C), (int)(2 * C)}};
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(256), 0, (hipStream_t)stream, ws, norm_grid(a.rows, a.C, true), (long)(2 * C), sg);
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(SUM_THREADS), 0, (hipStream_t)stream, ws, norm_grid(a.rows, a.C, true), (long)(2 * C), sg);
     return check_launch("layer_norm_bwd sums");
 }

@@ -738,19 +738,27 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(ScanArgs a) {
     }
 }
 
-// dB, dC [T][B][N] = the channel blocks' partial sums; behind them (blocks >= nbc) da_log, dskip, ddelta_bias += the (clip, run) rows'
+// dB, dC [T][B][N] = the channel blocks' partial sums (blocks from nsum on); in front of them da_log, dskip, ddelta_bias += the (clip, run)
+// rows'
 template <class S>
-__global__ __launch_bounds__(256) void scan_sum_kernel(const float* bc, S* db, S* dc, int parts, long long frames, int N, int NP, unsigned nbc,
-                                                       const float* sums, int P, long W, SumSegs sg) {
-    __shared__ double red[16 * 17];
-    if (blockIdx.x >= nbc) {
-        sum_partials(sums, P, W, sg, (blockIdx.x - nbc) * 16, red);
+__global__ __launch_bounds__(SUM_THREADS) void scan_sum_kernel(const float* bc, S* db, S* dc, int parts, long long frames, int N, int NP,
+                                                               const float* sums, int P, long W, unsigned nsum, SumSegs sg) {
+    __shared__ double red[SUM_LDS];
+    if (blockIdx.x < nsum) {
+        sum_partials(sums, P, W, sg, blockIdx.x * 16, red);
         return;
     }
     const long long n = frames * 2 * NP;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)nbc * 256) {
+    for (long long i = (long long)(blockIdx.x - nsum) * SUM_THREADS + threadIdx.x; i < n; i += (long long)(gridDim.x - nsum) * SUM_THREADS) {
         float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += bc[p * n + i];
+        int p = 0;
+        for (; p + 8 <= parts; p += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = bc[(p + k) * n + i];
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
+        for (; p < parts; ++p) s += bc[p * n + i];
         const long long f = i / (2 * NP);
         const int m = (int)(i % (2 * NP)), k = m % NP;
         if (k < N) (m < NP ? db : dc)[f * N + k] = (S)s;
@@ -758,38 +766,54 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* bc, S* db, S
 }
 
 // ------------------------------------------------------------------------------------------------ one frame
-// u, delta, z [B][D] and b, c [B][N] at clip strides, state [B][D][N] float -> state_out (which may be the same memory)
-template <class S, int LN, int NS>
+// u, delta, z [B][D] and b, c [B][N] at clip strides, state [B][D][N] float -> state_out (which may be the same memory).  Bound: HBM (the
+// states in and out).  LN lanes of four states share a channel; a block keeps the rates of its channels over `run` clips, and the next
+// clip's states are on their way while one is computed.  WHOLE: N is a multiple of four.
+template <class S, int LN, bool WHOLE>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
-    constexpr int CB = 256 / LN;
-    const int nq = threadIdx.x % LN, b = blockIdx.y, dd = blockIdx.x * CB + threadIdx.x / LN;
-    const bool on = dd < a.D;
-    const int d = on ? dd : 0;                                   // (every lane takes part in the sum)
-    const long long s0 = ((long long)b * a.D + d) * a.N;
-    float h[NS], al[NS], Bv[NS], Cv[NS];
-    load_states<NS>(a.h0 + s0, nq * NS, a.N, h);
-    load_states<NS>(a.a_log + (long long)d * a.N, nq * NS, a.N, al);
+    constexpr int CB = 256 / LN, NS = 4;
+    const int n0 = threadIdx.x % LN * NS, dd = blockIdx.x * CB + threadIdx.x / LN;
+    const int b0 = blockIdx.y * a.run, b1 = min(b0 + a.run, a.B);
+    const bool on = dd < a.D, has = n0 < a.N;
+    const int d = on ? dd : 0;                                   // (every lane takes part in the sums)
+    auto four = [&](const float* row, float (&v)[NS]) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        const bool has = nq * NS + j < a.N;
-        Bv[j] = has ? (float)static_cast<const S*>(a.b)[b * a.bb + nq * NS + j] : 0.f;
-        Cv[j] = has ? (float)static_cast<const S*>(a.c)[b * a.cb + nq * NS + j] : 0.f;
-    }
-    const float u = (float)static_cast<const S*>(a.u)[b * a.ub + d];
-    const float dt = step_of(a, (float)static_cast<const S*>(a.delta)[b * a.eb + d] + (a.dbias ? a.dbias[d] : 0.f));
-    const float z = a.z ? (float)static_cast<const S*>(a.z)[b * a.zb + d] : 0.f;
-    float y = 0.f;
+            for (int j = 0; j < NS; ++j) v[j] = 0.f;
+            if (has) load_loose<float, NS>(row + n0, v);
+        } else load_states<NS>(row, n0, a.N, v);
+    };
+    float A2[NS], h[NS], nxt[NS];
+    four(a.h0 + ((long long)b0 * a.D + d) * a.N, nxt);
+    four(a.a_log + (long long)d * a.N, A2);
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        h[j] = fmaf(__builtin_amdgcn_exp2f(dt * (-LOG2E * rate_of(al[j]))), h[j], dt * u * Bv[j]);
-        y = fmaf(Cv[j], h[j], y);
-    }
-    y = lanes_sum<LN>(y);
-    if (!on) return;
-    store_states<NS>(a.h_out + s0, nq * NS, a.N, h);
-    if (nq == 0) {
-        y = fmaf(a.skip ? a.skip[d] : 0.f, u, y);
-        static_cast<S*>(a.y)[(long long)b * a.D + d] = (S)(a.z ? y * (z * fast_sigmoid(z)) : y);
+    for (int j = 0; j < NS; ++j) A2[j] = -LOG2E * rate_of(A2[j]);
+    const float bias = a.dbias ? a.dbias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    for (int b = b0; b < b1; ++b) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) h[j] = nxt[j];
+        if (b + 1 < b1) four(a.h0 + ((long long)(b + 1) * a.D + d) * a.N, nxt);
+        const float u = (float)static_cast<const S*>(a.u)[b * a.ub + d], z = a.z ? (float)static_cast<const S*>(a.z)[b * a.zb + d] : 0.f;
+        const float dt = step_of(a, (float)static_cast<const S*>(a.delta)[b * a.eb + d] + bias), du = dt * u;
+        float y = 0.f;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const bool in = WHOLE ? has : n0 + j < a.N;
+            const float Bv = in ? (float)static_cast<const S*>(a.b)[b * a.bb + n0 + j] : 0.f, Cv = in ? (float)static_cast<const S*>(a.c)[b * a.cb + n0 + j] : 0.f;
+            h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], du * Bv);
+            y = fmaf(Cv, h[j], y);
+        }
+        y = lanes_sum<LN>(y);
+        if (on) {
+            float* out = a.h_out + ((long long)b * a.D + d) * a.N;
+            if constexpr (WHOLE) {
+                if (has) store_loose<float, NS>(out + n0, h);
+            } else store_states<NS>(out, n0, a.N, h);
+            if (n0 == 0) {
+                y = fmaf(skip, u, y);
+                static_cast<S*>(a.y)[(long long)b * a.D + d] = (S)(a.z ? y * (z * fast_sigmoid(z)) : y);
+            }
+        }
     }
 }
 
@@ -866,9 +890,15 @@ static int scan_bwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     hipLaunchKernelGGL((scan_bwd_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun), dim3(256), lds, s, a);
     return check_launch("selective_scan_bwd");
 }
-template <class S, int LN, int NS>
-static int scan_step_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
-    hipLaunchKernelGGL((scan_step_kernel<S, LN, NS>), dim3(p.blocks, a.B), dim3(256), 0, s, a);
+template <class S, int LN>
+static int scan_step_launch(ScanArgs& a, hipStream_t s) {
+    const int blocks = (a.D + 256 / LN - 1) / (256 / LN);
+    // clips per block: as many as leave every CU eight blocks
+    const long long runs = (long long)blocks * a.B / (8ll * device_cus());
+    a.run = runs < 1 ? 1 : runs > 64 ? 64 : (int)runs;
+    const dim3 grid(blocks, (a.B + a.run - 1) / a.run);
+    if (a.N % 4) hipLaunchKernelGGL((scan_step_kernel<S, LN, false>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((scan_step_kernel<S, LN, true>), grid, dim3(256), 0, s, a);
     return check_launch("selective_scan_step");
 }
 
@@ -961,10 +991,10 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
     if (rc) return rc;
     const long W = (long)D * (N + 2);
     const SumSegs sg{{da_log, dskip, ddelta_bias}, {D * N, D * (N + 1), D * (N + 2)}};
-    const long long n = (long long)T * B * 2 * p.np, most = 8ll * device_cus();
-    const unsigned nbc = (unsigned)((n + 255) / 256 < most ? (n + 255) / 256 : most), nsum = a.sums ? (unsigned)((W + 15) / 16) : 0;
-    PBSED_ELEM(dtype, hipLaunchKernelGGL(scan_sum_kernel<S>, dim3(nbc + nsum), dim3(256), 0, s, a.bc, static_cast<S*>(db), static_cast<S*>(dc),
-                                         p.blocks, (long long)T * B, N, p.np, nbc, a.sums, B * p.nrun, W, sg));
+    const long long n = (long long)T * B * 2 * p.np, most = 2ll * device_cus(), need = (n + SUM_THREADS - 1) / SUM_THREADS;
+    const unsigned nbc = (unsigned)(need < most ? need : most), nsum = a.sums ? (unsigned)((W + 15) / 16) : 0;
+    PBSED_ELEM(dtype, hipLaunchKernelGGL(scan_sum_kernel<S>, dim3(nsum + nbc), dim3(SUM_THREADS), 0, s, a.bc, static_cast<S*>(db), static_cast<S*>(dc),
+                                         p.blocks, (long long)T * B, N, p.np, a.sums, B * p.nrun, W, nsum, sg));
     return check_launch("selective_scan_bwd sums");
 }
 
@@ -974,13 +1004,13 @@ extern "C" int pbsed_selective_scan_step(const void* u, const void* delta, const
                                          const long long* strides /*host*/, int B, int D, int N, int softplus, int dtype, void* stream) {
     if (const int rc = scan_check("selective_scan_step", 1, B, D, N, dtype)) return rc;
     if (!u || !delta || !a_log || !b || !c || !state || !state_out || !y || !strides) { set_error("selective_scan_step: null pointer"); return PBSED_E_ARG; }
-    const ScanPlan p = scan_plan(1, B, D, N, false);
     ScanArgs a{};
     a.u = u; a.delta = delta; a.a_log = a_log; a.b = b; a.c = c; a.skip = skip; a.z = z; a.dbias = delta_bias; a.h0 = state; a.h_out = state_out; a.y = y;
     a.ub = strides[0]; a.eb = strides[1]; a.bb = strides[2]; a.cb = strides[3]; a.zb = strides[4];
     a.B = B; a.D = D; a.N = N; a.softplus = softplus;
     hipStream_t s = (hipStream_t)stream;
     int rc = PBSED_OK;
-    PBSED_SCAN(scan_step_launch);
+    PBSED_ELEM(dtype, rc = N <= 4 ? scan_step_launch<S, 1>(a, s) : N <= 8 ? scan_step_launch<S, 2>(a, s) : N <= 16 ? scan_step_launch<S, 4>(a, s)
+                          : N <= 32 ? scan_step_launch<S, 8>(a, s) : scan_step_launch<S, 16>(a, s));
     return rc;
 }

@@ -1489,15 +1489,13 @@ def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=
     return dx, dstate
 
 
-def _step_state(name, state, state_out, ps, shape, dtype, dev, **inputs):
+def _step_state(name, state, state_out, ps, shape, dtype, dev):
     """Address of where a one-frame form leaves its state: in place, or a buffer that does not overlap what it reads."""
     if state_out is None or state_out is state:
         return ps
     po = _like(name, 'state_out', state_out, shape, dtype, dev, True)
-    if po != ps:
-        lo, hi = po, po + _span(state_out)
-        if ps < hi and lo < ps + _span(state):
-            _fail(name, 'state_out overlaps state')
+    if po != ps and abs(po - ps) < state.nbytes:
+        _fail(name, 'state_out overlaps state')
     return po
 
 
