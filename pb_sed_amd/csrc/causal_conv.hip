@@ -23,7 +23,7 @@ struct CConvArgs {
     int T, B, D, reverse, silu, ts, nrun;       // ts: positions per run; nrun: runs per clip
 };
 
-constexpr int CC_G = 8;                         // positions per load group
+constexpr int CC_G = 8, CC_BG = 4;              // positions per load group, forward and backward
 
 template <class S, int V>
 __device__ __forceinline__ void zero_v(float (&v)[V]) {
@@ -90,12 +90,24 @@ __global__ __launch_bounds__(256) void causal_conv_fwd_kernel(CConvArgs a) {
     };
     int p = p0;
     const int valid = min(p1, len);
+    LoosePack<S, V> nxt[CC_G];                  // the next group on its way, in its own type
+    auto fetch = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < CC_G; ++i) nxt[i] = *reinterpret_cast<const LoosePack<S, V>*>(x + frame(q + i) * a.xt);
+    };
+    if (p + CC_G <= valid) fetch(p);
     for (; p + CC_G <= valid; p += CC_G) {
-        float cur[CC_G][V];
+        LoosePack<S, V> now[CC_G];
 #pragma unroll
-        for (int i = 0; i < CC_G; ++i) load_loose<S, V>(x + frame(p + i) * a.xt, cur[i]);
+        for (int i = 0; i < CC_G; ++i) now[i] = nxt[i];
+        if (p + 2 * CC_G <= valid) fetch(p + CC_G);
 #pragma unroll
-        for (int i = 0; i < CC_G; ++i) one(p + i, cur[i]);
+        for (int i = 0; i < CC_G; ++i) {
+            float cur[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) cur[v] = (float)now[i].v[v];
+            one(p + i, cur);
+        }
     }
     for (; p < valid; ++p) {
         float cur[V];
@@ -191,15 +203,27 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CConvArgs a) {
         };
         int q = p0;
         if (valid > p0 || run == 0) {
-            for (; q + CC_G <= valid; q += CC_G) {
-                float cur[CC_G][V], g[CC_G][V];
+            LoosePack<S, V> nx[CC_BG], ng[CC_BG];
+            auto fetch = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < CC_G; ++i) {
-                    load_loose<S, V>(x + frame(q + i) * a.xt, cur[i]);
-                    load_loose<S, V>(dy + frame(q + i) * a.gt, g[i]);
+                for (int i = 0; i < CC_BG; ++i) {
+                    nx[i] = *reinterpret_cast<const LoosePack<S, V>*>(x + frame(p + i) * a.xt);
+                    ng[i] = *reinterpret_cast<const LoosePack<S, V>*>(dy + frame(p + i) * a.gt);
                 }
+            };
+            if (q + CC_BG <= valid) fetch(q);
+            for (; q + CC_BG <= valid; q += CC_BG) {
+                LoosePack<S, V> px[CC_BG], pg[CC_BG];
 #pragma unroll
-                for (int i = 0; i < CC_G; ++i) one(q + i, cur[i], g[i], true);
+                for (int i = 0; i < CC_BG; ++i) { px[i] = nx[i]; pg[i] = ng[i]; }
+                if (q + 2 * CC_BG <= valid) fetch(q + CC_BG);
+#pragma unroll
+                for (int i = 0; i < CC_BG; ++i) {
+                    float cur[V], g[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) { cur[v] = (float)px[i].v[v]; g[v] = (float)pg[i].v[v]; }
+                    one(q + i, cur, g, true);
+                }
             }
             // the rest of the run and the K - 1 positions behind it (zeros behind the clip's end)
             const int stop = max(valid, p0) + K - 1;
@@ -273,7 +297,7 @@ static void cconv_launch3(const CConvArgs& a, bool bwd, hipStream_t s) {
     const long long units = (long long)a.B * a.nrun;
     const dim3 grid((a.D + 64 * V - 1) / (64 * V), (unsigned)((units + CC_RB - 1) / CC_RB));
     if (bwd) {
-        if constexpr (V <= 4) hipLaunchKernelGGL((causal_conv_bwd_kernel<S, V, K>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((causal_conv_bwd_kernel<S, V, K>), grid, dim3(256), 0, s, a);
     } else hipLaunchKernelGGL((causal_conv_fwd_kernel<S, V, K>), dim3((unsigned)((units * grid.x + 3) / 4)), dim3(256), 0, s, a);
 }
 template <class S, int V>
@@ -290,12 +314,11 @@ static void cconv_launch2(const CConvArgs& a, int K, bool bwd, hipStream_t s) {
 }
 template <class S>
 static int cconv_launch(CConvArgs& a, int K, bool bwd, hipStream_t s) {
-    const int full = bwd ? 4 : 16 / (int)sizeof(S), v = a.D >= full ? full : 1;
+    const int full = 4, v = a.D >= full ? full : 1;
     a.ts = cconv_ts(a.T, a.B, a.D, v);
     a.nrun = (a.T + a.ts - 1) / a.ts;
     if (v == 1) cconv_launch2<S, 1>(a, K, bwd, s);
-    else if (bwd) cconv_launch2<S, 4>(a, K, bwd, s);
-    else cconv_launch2<S, 16 / sizeof(S)>(a, K, bwd, s);
+    else cconv_launch2<S, 4>(a, K, bwd, s);
     return check_launch(bwd ? "causal_conv_bwd" : "causal_conv_fwd");
 }
 

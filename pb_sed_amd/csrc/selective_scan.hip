@@ -34,7 +34,7 @@ struct ScanArgs {
     float* bc;                                         // backward: [channel blocks][T][B][2 NP] partial sums of dB | dC
     float* sums;                                       // backward: [B nrun][D N + 2 D] partial sums of da_log | dskip | ddelta_bias
     long long ut, ub, et, eb, bt, bb, ct, cb, zt, zb, gt, gb, dzt, dzb;      // strides over frames and clips (elements)
-    int T, B, D, N, reverse, softplus, nrun, run;      // run: frames per run, a multiple of 64
+    int T, B, D, N, reverse, softplus, nrun, run;      // run: frames per run, a number of tiles
     int folded;                                        // runs hold the states in front of the runs (scan_runs_kernel has been there)
 };
 
@@ -489,7 +489,7 @@ template <int LN, int NS> struct ScanBwdLds {
     static constexpr size_t bytes = (size_t)(3 * rows + 2 * bc + part + keep) * sizeof(float);
 };
 template <class S, int LN, int NS>
-__global__ __launch_bounds__(256, 2) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
     using L = ScanBwdLds<LN, NS>;
     constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F;                  // F frames of a channel per thread and tile
     constexpr int NP2 = TT * 2 * NP / 256;
@@ -635,17 +635,11 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(ScanArgs a) {
             if (k + 1 < TT / 4) gr = next;
         }
         float dat[NS] = {};
-        ScanGroup<NS, true> gb;
-        float4 g4 = *reinterpret_cast<const float4*>(rowG + TT - 4);
-        gb.template load<NP>(rowD, rowU, sB, sC, TT / 4 - 1, nq);
 #pragma unroll
         for (int k = TT / 4 - 1; k >= 0; --k) {
-            ScanGroup<NS, true> next;
-            float4 gn = g4;
-            if (k) {
-                next.template load<NP>(rowD, rowU, sB, sC, k - 1, nq);
-                gn = *reinterpret_cast<const float4*>(rowG + 4 * (k - 1));
-            }
+            ScanGroup<NS, true> gb;
+            gb.template load<NP>(rowD, rowU, sB, sC, k, nq);
+            const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
             __builtin_amdgcn_sched_barrier(0);
             float yo[4], bo[4], ko[4];
 #pragma unroll
@@ -683,7 +677,6 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(ScanArgs a) {
                 store_pack<float, 4>(rowU + 4 * k, bo);
                 store_pack<float, 4>(rowG + 4 * k, yo);
             }
-            if (k) { gb = next; g4 = gn; }
         }
 #pragma unroll
         for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (sums over a tile first: long clips keep their digits)
@@ -824,9 +817,11 @@ struct ScanPlan {
     long long o_dt, o_bc, o_sums;                        // offsets in the workspace
 };
 // Frames are cut into runs where channel blocks x clips leave CUs with hardly more than one block: a lone block per CU is bound by the
-// latency of its chain, and a cut costs the first launch (about 0.7 of the main one's work).  Measured: 192 blocks, T 1001, bf16: forward
-// 82 us uncut, 64 in 4 runs, 63 in 8, 89 in 16; backward 224, 155, 143, 168.  512 blocks, T 500, float: 50 uncut, 66 in 2; backward 146,
-// 163.  16 blocks, T 40000: 694 us in 8, 202 in 64, 188 in 256.
+// latency of its chain, and a cut costs the first launch (about 0.7 of the main one's work).  Up to SC_FOLD runs the main launch folds
+// those in front of its own by itself; more are folded by scan_runs_kernel, whose cost grows with the channels.  Measured (forward,
+// backward us): 192 blocks, T 1001, bf16: 83, 233 uncut; 64, 135 in 4 runs; 62, 127 in 5; 63, 135 in 8; 98, 173 in 32.  512 blocks, T 500,
+// float: 51, 148 uncut; 67, 148 in 2.  16 blocks, T 40000: 357 in 16; 205 in 64; 193 in 128; 192 in 250.  20 blocks, T 313: 34 uncut, 20 in 7.
+constexpr int SC_FOLD = 16;
 static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     ScanPlan p{};
     p.ln = N <= 8 ? 4 : N <= 16 ? 8 : 16;
@@ -835,11 +830,14 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     p.cb = 256 / p.ln;
     p.blocks = (D + p.cb - 1) / p.cb;
     const long long have = (long long)p.blocks * B, cus = device_cus();
-    p.run = (T + 63) / 64 * 64;
+    const int grain = p.cb >= 64 ? 16 : 1024 / p.cb, least = grain < 24 ? 48 : 2 * grain;     // a run is a number of (forward) tiles
+    p.run = (T + grain - 1) / grain * grain;
     if (have * 8 <= cus * 9) {
-        long long runs = (5 * cus + have - 1) / have;
+        long long runs = 4 * cus / have;
+        if (runs > SC_FOLD) runs = 8 * cus / have;
         if (runs > 256) runs = 256;
-        p.run = (int)(((T + runs - 1) / runs + 63) / 64 * 64);
+        const int len = (int)(((T + runs - 1) / runs + grain - 1) / grain * grain);
+        p.run = len > least ? len : least;
     }
     p.nrun = (T + p.run - 1) / p.run;
     p.saved = (long long)((T + SC_SAVE - 1) / SC_SAVE) * B * D * p.np;
@@ -860,7 +858,6 @@ static int scan_check(const char* name, int T, int B, int D, int N, int dtype) {
     return PBSED_OK;
 }
 
-constexpr int SC_FOLD = 8;                               // up to so many runs the main launch folds those in front of its own by itself
 static int scan_fold(ScanArgs& a, const ScanPlan& p, int back, hipStream_t s) {
     a.folded = p.nrun > SC_FOLD;
     if (!a.folded) return PBSED_OK;

@@ -21,6 +21,6 @@ void set_error(const char* fmt, ...) {
     va_end(ap);
 }
 int check_launch(const char*) { return 0; }
-int device_cus() { return 4; }
+int device_cus() { return 8; }
 }  // namespace pbsed
 extern "C" const char* emu_last_error() { return pbsed::g_err; }
