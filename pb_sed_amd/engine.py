@@ -546,6 +546,17 @@ def _wgrad_job(jobs, dg, x, shift, dw, db):
         lst.append(v)
 
 
+def dropout_state(wrapper, device):
+    """The (seed, step) of a training pass's masks between the layers of ``wrapper``, on the device.  The seed comes from torch's CPU
+    generator at the first pass (torch.manual_seed governs it; ranks that shall draw different masks seed it differently), the step
+    counts the passes."""
+    if wrapper.dropout_rng is None or wrapper.dropout_rng.device != device:
+        wrapper.dropout_rng = ops.host_to_device(np.array([torch.randint(1 << 62, ()).item(), 0]), device, torch.int64)
+    now = wrapper.dropout_rng.clone()
+    wrapper.dropout_rng[1] += 1
+    return now
+
+
 def _scan_as_stack(wrappers):
     return wrappers[0].hidden_size in (64, 128, 256, 512)
 
@@ -562,7 +573,13 @@ def rnn_forward(wrappers, h, seq_dev, seq_host, training, precision='f32', h_tbc
     chains = _chains(wrappers)
     num_layers = wrappers[0].num_layers
     assert all(w.num_layers == num_layers for w in wrappers)
-    if h is not None and not any(w.bidirectional for w in wrappers) and wrappers[0].hidden_size in (64, 128, 256, 512) \
+    # dropout between the layers (training): the layer-by-layer path, masks from (seed, step) and the site layer * 8 + chain
+    masks = [dropout_state(w, (h if h is not None else h_tbc).device) if training and w.dropout else None for w in wrappers]
+
+    def dropped(x, l, i):
+        w = chains[i].widx
+        return x if masks[w] is None else ops.dropout(x, wrappers[w].dropout, masks[w], site=8 * l + i)
+    if h is not None and all(m is None for m in masks) and not any(w.bidirectional for w in wrappers) and wrappers[0].hidden_size in (64, 128, 256, 512) \
             and all(w.rnn.input_size == h.shape[1] for w in wrappers):
         return _stack_rnn_forward(wrappers, chains, h, seq_dev, seq_host, training, precision, h_tbc)
     of_w = [[i for i, ch in enumerate(chains) if ch.widx == wi] for wi in range(len(wrappers))]
@@ -607,21 +624,21 @@ def rnn_forward(wrappers, h, seq_dev, seq_host, training, precision='f32', h_tbc
         else:
             hs, save = ops.gru_scan_fwd(gi, w_hh_l, b_hh_l, [ch.reverse for ch in chains], seq_dev, save=training)
         layer_ctx.append((src, pcs, hs, save))
-        src = [[hs[i] for i in of_w[wi]] for wi in range(len(wrappers))]
+        src = [[hs[i] if l + 1 == num_layers else dropped(hs[i], l, i) for i in of_w[wi]] for wi in range(len(wrappers))]
     # the heads take the top layer's states in the scans' layout (both directions side by side)
     top = []
     for wi, w in enumerate(wrappers):
         outs = [hs[i] for i in of_w[wi]]
         top.append(outs[0] if len(outs) == 1 else torch.cat(outs, dim=2))
     logits, head_ctx = _heads_forward(wrappers, [None] * len(wrappers), seq_dev, seq_host, training, precision, x_tbc=top)
-    return logits, (chains, layer_ctx, head_ctx, precision, h)
+    return logits, (chains, layer_ctx, head_ctx, precision, h, dropped)
 
 
 def rnn_backward(wrappers, ctx, dlogits, seq_dev, seq_host):
     """Returns grad wrt the shared input h."""
     if ctx[0] == 'stack':
         return _stack_rnn_backward(wrappers, ctx, dlogits, seq_dev, seq_host)
-    chains, layer_ctx, head_ctx, precision, h = ctx
+    chains, layer_ctx, head_ctx, precision, h, dropped = ctx
     num_layers = wrappers[0].num_layers
     hid = wrappers[0].hidden_size
     of_w = [[i for i, ch in enumerate(chains) if ch.widx == wi] for wi in range(len(wrappers))]
@@ -695,7 +712,8 @@ def rnn_backward(wrappers, ctx, dlogits, seq_dev, seq_host):
                 gp = _gemm_prec(precision, w_t[0].shape[1])
                 if l > 0:                            # straight into the per-chain gradients of the layer below
                     for k, i in enumerate(mine):
-                        new_dy[i] = ops.tm_gemm([dgi[j] for j in mine], [w[k * hid:(k + 1) * hid] for w in w_t], None, gp, role='bwd')
+                        new_dy[i] = dropped(ops.tm_gemm([dgi[j] for j in mine], [w[k * hid:(k + 1) * hid] for w in w_t], None, gp, role='bwd'),
+                                            l - 1, i)
                 else:
                     d = ops.tbc_to_bct(ops.tm_gemm([dgi[j] for j in mine], w_t, None, gp, role='bwd'))
                     dh_in = d if dh_in is None else dh_in.add_(d)

@@ -82,15 +82,15 @@ class CRNN(SoundEventModel):
 
     @classmethod
     def build(cls, num_events=10, number_of_filters=128, stft_size=1024, sample_rate=16000,
-              hidden_size=256, num_layers=2, net=None, tag_conditioning=True, **kw):
+              hidden_size=256, num_layers=2, net=None, tag_conditioning=True, rnn_dropout=0., **kw):
         """Reference factory (pb_sed/experiments/strong_label_crnn/training.py:159-263,
-        pb_sed/models/strong_label/crnn.py:155-197)."""
+        pb_sed/models/strong_label/crnn.py:155-197).  ``rnn_dropout``: dropout between the GRU layers (torch.nn.GRU's ``dropout``)."""
         net = dict(SHALLOW if net is None else net)
         fe = NormalizedLogMelExtractor(sample_rate, stft_size, number_of_filters)
         cd = num_events if tag_conditioning else 0
         cnn = build_cnn(1, input_height=number_of_filters, conditional_dims=cd, **net)
         rnn = build_rnn(net['out_channels_1d'][-1] + cd, hidden_size, num_layers, num_events, hidden_size,
-                        bidirectional=True)
+                        bidirectional=True, dropout=rnn_dropout)
         return cls(fe, cnn, rnn, tag_conditioning=tag_conditioning, **kw)
 
     @classmethod

@@ -102,16 +102,17 @@ class CRNN(SoundEventModel):
 
     @classmethod
     def build(cls, num_events=10, number_of_filters=128, stft_size=1024, sample_rate=16000,
-              hidden_size=256, num_layers=2, net=None, rnn_bwd=True, feature_extractor=None, **kw):
+              hidden_size=256, num_layers=2, net=None, rnn_bwd=True, feature_extractor=None, rnn_dropout=0., **kw):
         """Reference model factory (pb_sed/experiments/weak_label_crnn/training.py:158-260).  ``feature_extractor``:
         extra NormalizedLogMelExtractor fields, e.g. the training augmentation of training.py:209-216
-        (dict(n_time_masks=1, n_frequency_masks=1, max_noise_scale=.2))."""
+        (dict(n_time_masks=1, n_frequency_masks=1, max_noise_scale=.2)).  ``rnn_dropout``: dropout between the GRU layers
+        (torch.nn.GRU's ``dropout``)."""
         net = dict(SHALLOW if net is None else net)
         fe = NormalizedLogMelExtractor(sample_rate, stft_size, number_of_filters, **(feature_extractor or {}))
         cnn = build_cnn(1, input_height=number_of_filters, **net)
         c = net['out_channels_1d'][-1]
-        fwd = build_rnn(c, hidden_size, num_layers, num_events, hidden_size)
-        bwd = build_rnn(c, hidden_size, num_layers, num_events, hidden_size, reverse=True) if rnn_bwd else None
+        fwd = build_rnn(c, hidden_size, num_layers, num_events, hidden_size, dropout=rnn_dropout)
+        bwd = build_rnn(c, hidden_size, num_layers, num_events, hidden_size, reverse=True, dropout=rnn_dropout) if rnn_bwd else None
         return cls(fe, cnn, fwd, bwd, **kw)
 
     @classmethod

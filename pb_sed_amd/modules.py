@@ -424,9 +424,10 @@ class GRU(nn.Module):
         super().__init__()
         if not isinstance(rnn, nn.GRU):
             raise NotImplementedError(f'recurrent part must be a torch.nn.GRU, got {type(rnn).__name__}')
-        if not rnn.bias or not rnn.batch_first or rnn.dropout:
-            raise NotImplementedError('torch.nn.GRU(bias=True, batch_first=True, dropout=0) is what the kernels implement')
+        if not rnn.bias or not rnn.batch_first or not 0. <= rnn.dropout < 1.:
+            raise NotImplementedError('torch.nn.GRU(bias=True, batch_first=True, 0 <= dropout < 1) is what the kernels implement')
         self.rnn, self.output_net, self.reverse = rnn, output_net, reverse
+        self.dropout_rng = None       # int64 [seed, step] of the masks between the layers (engine.dropout_state), no part of the checkpoint
         if rnn.hidden_size % 64:
             raise NotImplementedError('GRU hidden size must be a multiple of 64')
 
@@ -434,6 +435,7 @@ class GRU(nn.Module):
     hidden_size = property(lambda self: self.rnn.hidden_size)
     num_layers = property(lambda self: self.rnn.num_layers)
     bidirectional = property(lambda self: self.rnn.bidirectional)
+    dropout = property(lambda self: self.rnn.dropout if self.rnn.num_layers > 1 else 0.)      # torch.nn.GRU: behind every layer but the last
 
     @classmethod
     def finalize_dogmatic_config(cls, config):
@@ -485,9 +487,9 @@ def build_cnn(in_channels, out_channels_2d, pool_sizes_2d, kernel_size_2d, out_c
 
 
 def build_rnn(input_size, hidden_size, num_layers, num_events, head_hidden, bidirectional=False,
-              reverse=False, eps=1e-3):
+              reverse=False, eps=1e-3, dropout=0.):
     dirs = 2 if bidirectional else 1
     output_net = CNN1d(hidden_size * dirs, [head_hidden, num_events], 1, 1, eps=eps, pre_activation=False,
                        output_layer=True)
-    rnn = nn.GRU(input_size, hidden_size, num_layers, bias=True, batch_first=True, dropout=0., bidirectional=bidirectional)
+    rnn = nn.GRU(input_size, hidden_size, num_layers, bias=True, batch_first=True, dropout=dropout, bidirectional=bidirectional)
     return GRU(rnn, output_net, reverse)
