@@ -1389,6 +1389,25 @@ def _on_device(dev, fn, *args):
         return fn(*args)
 
 
+_SIZES = {}             # (entry point, device, sizes) -> its answer
+
+
+def _floats(entry, dev, *sizes):
+    """Workspace of a call: a function of its sizes and of the device alone, asked for once."""
+    key = (entry, dev, sizes)
+    floats = _SIZES.get(key)
+    if floats is None:
+        if len(_SIZES) > 4096:
+            _SIZES.clear()
+        floats = _SIZES[key] = _on_device(dev, getattr(_lib.lib(), entry), *sizes)
+    return floats
+
+
+def _empty(x, shape):
+    """A new contiguous tensor of the type and device of x, whose shape it has."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format) if x.is_contiguous() else x.new_empty(shape)
+
+
 def _strides(*tensors):
     """(frame stride, clip stride) of every [T, B, channels] tensor (None: zeros), as the host array of the C-ABI."""
     vals = []
@@ -1449,7 +1468,7 @@ def causal_conv_fwd(x, weight, bias=None, *, silu=True, seq_len=None, reverse=Fa
     pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
     pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
     ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
-    y = x.new_empty(shape)
+    y = _empty(x, shape)
     state_out = x.new_empty((b, k - 1, d)) if want_state else None
     st, sb, _ = x.stride()
     _launch(dev, 'pbsed_causal_conv_fwd', px, pw, pb, pl, ps, y.data_ptr(), state_out.data_ptr() if want_state else None, t, b, d, k, st, sb,
@@ -1474,12 +1493,12 @@ def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=
     ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
     pso = _like(name, 'dstate_out', dstate_out, (b, k - 1, d), x.dtype, dev, True)
     if dx is None:
-        dx = x.new_empty(shape)
+        dx = _empty(x, shape)
     else:
         _like(name, 'dx', dx, shape, x.dtype, dev)
         _distinct(name, 'dx', dx, x=x, dy=dy, state=state, dstate_out=dstate_out)
     dstate = x.new_empty((b, k - 1, d)) if want_dstate else None
-    floats = _on_device(dev, _lib.lib().pbsed_causal_conv_workspace, t, b, d, k) if pdw or pdb else 0
+    floats = _floats('pbsed_causal_conv_workspace', dev, t, b, d, k) if pdw or pdb else 0
     ws = x.new_empty(floats, dtype=torch.float32) if floats else None
     gt, gb, _ = dy.stride()
     xt, xb, _ = x.stride()
@@ -1509,7 +1528,7 @@ def causal_conv_step(x, weight, bias, state, *, silu=True, state_out=None):
     pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
     ps = _have(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
     po = _step_state(name, state, state_out, ps, (b, k - 1, d), x.dtype, dev)
-    y = x.new_empty(shape)
+    y = _empty(x, shape)
     _launch(dev, 'pbsed_causal_conv_step', px, pw, pb, ps, po, y.data_ptr(), b, d, k, x.stride(0), int(silu), code)
     return y
 
@@ -1555,7 +1574,7 @@ def selective_scan_fwd(u, delta, a_log, b, c, *, d=None, z=None, delta_bias=None
     pl = _like(name, 'seq_len', seq_len, (bs,), torch.int32, dev, True)
     ps = _like(name, 'state', state, (bs, width, n), torch.float32, dev, True)
     n_saved, n_ws = _scan_plan(dev, t, bs, width, n, False)
-    y = u.new_empty((t, bs, width))
+    y = _empty(u, u.shape)
     state_out = u.new_empty((bs, width, n), dtype=torch.float32) if want_state else None
     saved = u.new_empty(n_saved, dtype=torch.float32) if save else None
     ws = u.new_empty(n_ws, dtype=torch.float32) if n_ws else None
@@ -1588,8 +1607,8 @@ def selective_scan_bwd(dy, u, delta, a_log, b, c, saved, *, d=None, z=None, delt
         _like(name, 'dz', dz, shape, u.dtype, dev)
         _distinct(name, 'dz', dz, dy=dy, u=u, delta=delta, z=z, b=b, c=c)
     elif z is not None:
-        dz = u.new_empty(shape)
-    du, ddelta = u.new_empty(shape), u.new_empty(shape)
+        dz = _empty(u, shape)
+    du, ddelta = _empty(u, shape), _empty(u, shape)
     db, dc = u.new_empty((t, bs, n)), u.new_empty((t, bs, n))
     dstate = u.new_empty((bs, width, n), dtype=f32) if want_dstate else None
     ws = u.new_empty(n_ws, dtype=f32)
@@ -1607,7 +1626,7 @@ def selective_scan_step(u, delta, a_log, b, c, state, *, d=None, z=None, delta_b
     bs, width = u.shape
     ps = _have(name, 'state', state, (bs, width, n), torch.float32, dev, True)
     po = _step_state(name, state, state_out, ps, (bs, width, n), torch.float32, dev)
-    y = u.new_empty((bs, width))
+    y = _empty(u, u.shape)
     strides = (C.c_longlong * 5)(u.stride(0), delta.stride(0), b.stride(0), c.stride(0), 0 if z is None else z.stride(0))
     _launch(dev, 'pbsed_selective_scan_step', *ptrs, ps, po, y.data_ptr(), strides, bs, width, n, int(softplus), code)
     return y
@@ -1615,6 +1634,8 @@ def selective_scan_step(u, delta, a_log, b, c, state, *, d=None, z=None, delta_b
 
 def _row_stride(name, what, v):
     """The one stride between the rows of a [..., C] tensor."""
+    if v.is_contiguous():
+        return v.shape[-1]
     shape, strides = v.shape, v.stride()
     c = shape[-1]
     row, rows = None, 1                                     # from the innermost axis outwards: every axis continues the one inside it
@@ -1646,7 +1667,7 @@ def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5, save=False):
     pb = _like(name, 'bias', bias, (c,), torch.float32, dev, True)
     if not eps >= 0:
         _fail(name, f'eps = {eps}')
-    y = x.new_empty(shape)
+    y = _empty(x, shape)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if save else None
     _launch(dev, 'pbsed_layer_norm_fwd', px, pw, pb, y.data_ptr(), stats.data_ptr() if save else None, rows, c, xs, float(eps), code)
     return y, stats
@@ -1665,8 +1686,8 @@ def layer_norm_bwd(dy, x, weight, stats, *, dweight=None, dbias=None):
     pst = _have(name, 'stats', stats, (rows, 2), torch.float32, dev, True)
     pdw = _like(name, 'dweight', dweight, (c,), torch.float32, dev, True)
     pdb = _like(name, 'dbias', dbias, (c,), torch.float32, dev, True)
-    dx = x.new_empty(shape)
-    floats = _on_device(dev, _lib.lib().pbsed_layer_norm_workspace, rows, c) if pdw or pdb else 0
+    dx = _empty(x, shape)
+    floats = _floats('pbsed_layer_norm_workspace', dev, rows, c) if pdw or pdb else 0
     ws = x.new_empty(floats, dtype=torch.float32) if floats else None
     _launch(dev, 'pbsed_layer_norm_bwd', pg, px, pw, pst, dx.data_ptr(), pdw, pdb, ws.data_ptr() if floats else None, floats, rows, c,
             _row_stride(name, 'dy', dy), _row_stride(name, 'x', x), code)
@@ -1690,7 +1711,7 @@ def dropout(x, p, rng, *, site=0, residual=None, out=None):
     pr = _have(name, 'rng', rng, (2,), torch.int64, dev, True)
     pres = _like(name, 'residual', residual, shape, x.dtype, dev)
     if out is None:
-        out = x.new_empty(shape)
+        out = _empty(x, shape)
     else:
         _like(name, 'out', out, shape, x.dtype, dev)
         same = {key: v for key, v in (('x', x), ('residual', residual))
