@@ -51,6 +51,69 @@ template <int LN> __device__ __forceinline__ float lanes_sum(float v) {         
     if constexpr (LN >= 16) v += dpp_lane<0x140>(v);     // row_mirror
     return v;
 }
+// Of K pairs (x, y): x stays in the banks (lanes 4 k .. 4 k + 3 of a row) outside MASK, y's sum over the two lanes of CTRL takes the banks
+// inside it.  The compiler has no form for an addition that writes some banks only; the waits are those of a lane exchange behind a
+// vector instruction, in front (it wrote y) and behind (an exchange reads x).
+#ifdef HIP_EMU
+#define SCAN_MERGE(K, CTRL, MASK, TEXT, ...)                                                                       \
+    for (int k = 0; k < K; ++k) {                                                                                  \
+        const float m = y[k] + dpp_lane<CTRL>(y[k]);                                                               \
+        x[k] = MASK >> ((threadIdx.x >> 2) & 3) & 1 ? m : x[k];                                                    \
+    }
+#else
+#define SCAN_MERGE(K, CTRL, MASK, TEXT, ...) asm("s_nop 1\n\t" TEXT "s_nop 1" __VA_ARGS__)
+#endif
+#define SCAN_ADD(X, Y, CTRL, MASK) "v_add_f32_dpp %" #X ", %" #Y ", %" #Y " " CTRL " row_mask:0xf bank_mask:" MASK "\n\t"
+template <int K> __device__ __forceinline__ void merge_ror8(float* x, const float* y) {
+    static_assert(K == 2 || K == 6, "");
+    if constexpr (K == 2) {
+        SCAN_MERGE(2, 0x128, 0xc, SCAN_ADD(0, 2, "row_ror:8", "0xc") SCAN_ADD(1, 3, "row_ror:8", "0xc"),
+                   : "+v"(x[0]), "+v"(x[1]) : "v"(y[0]), "v"(y[1]));
+    } else {
+        SCAN_MERGE(6, 0x128, 0xc, SCAN_ADD(0, 6, "row_ror:8", "0xc") SCAN_ADD(1, 7, "row_ror:8", "0xc") SCAN_ADD(2, 8, "row_ror:8", "0xc")
+                   SCAN_ADD(3, 9, "row_ror:8", "0xc") SCAN_ADD(4, 10, "row_ror:8", "0xc") SCAN_ADD(5, 11, "row_ror:8", "0xc"),
+                   : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5])
+                   : "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), "v"(y[4]), "v"(y[5]));
+    }
+}
+template <int K> __device__ __forceinline__ void merge_half(float* x, const float* y) {
+    static_assert(K == 1 || K == 2 || K == 3 || K == 6, "");
+    if constexpr (K == 1) {
+        SCAN_MERGE(1, 0x141, 0xa, SCAN_ADD(0, 1, "row_half_mirror", "0xa"), : "+v"(x[0]) : "v"(y[0]));
+    } else if constexpr (K == 2) {
+        SCAN_MERGE(2, 0x141, 0xa, SCAN_ADD(0, 2, "row_half_mirror", "0xa") SCAN_ADD(1, 3, "row_half_mirror", "0xa"),
+                   : "+v"(x[0]), "+v"(x[1]) : "v"(y[0]), "v"(y[1]));
+    } else if constexpr (K == 3) {
+        SCAN_MERGE(3, 0x141, 0xa, SCAN_ADD(0, 3, "row_half_mirror", "0xa") SCAN_ADD(1, 4, "row_half_mirror", "0xa") SCAN_ADD(2, 5, "row_half_mirror", "0xa"),
+                   : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]) : "v"(y[0]), "v"(y[1]), "v"(y[2]));
+    } else {
+        SCAN_MERGE(6, 0x141, 0xa, SCAN_ADD(0, 6, "row_half_mirror", "0xa") SCAN_ADD(1, 7, "row_half_mirror", "0xa") SCAN_ADD(2, 8, "row_half_mirror", "0xa")
+                   SCAN_ADD(3, 9, "row_half_mirror", "0xa") SCAN_ADD(4, 10, "row_half_mirror", "0xa") SCAN_ADD(5, 11, "row_half_mirror", "0xa"),
+                   : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5])
+                   : "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), "v"(y[4]), "v"(y[5]));
+    }
+}
+// Sums over a channel's LN lanes of Q quantities at four frames, v[quantity + Q * frame].  The lanes of a channel split the frames: every
+// step across banks halves the registers (Q = 3, LN = 8: 24 additions in place of 36).  Afterwards v[quantity + Q * i] holds frame
+// W (lane % LN / 4) + i of the W = lane_frames<LN> that the lane's bank keeps.
+template <int LN> constexpr int lane_frames = LN <= 4 ? 4 : 16 / LN;
+template <int LN, int Q> __device__ __forceinline__ void lanes_sum4(float (&v)[4 * Q]) {
+    constexpr int K = Q * lane_frames<LN>;
+    if constexpr (LN == 16) {
+#pragma unroll
+        for (int k = 0; k < 2 * Q; ++k) v[k] += dpp_lane<0x128>(v[k]);
+        merge_ror8<2 * Q>(v, v + 2 * Q);
+    }
+    if constexpr (LN >= 8) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += dpp_lane<0x141>(v[k]);
+        merge_half<K>(v, v + K);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += dpp_lane<0xB1>(v[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += dpp_lane<0x4E>(v[k]);
+}
 // the NS states from n0 on of a row of N floats (zeros behind N)
 template <int NS> __device__ __forceinline__ void load_states(const float* row, int n0, int N, float (&v)[NS]) {
 #pragma unroll
@@ -148,9 +211,19 @@ constexpr unsigned SC_OUT = 0x80000000u;
 template <class S> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const S* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(p), 0, 0x7fffffffu, 0x00020000);
 }
-template <class S> __device__ __forceinline__ float row_load(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff) {
+// Elements on their way stay as they are in memory: a conversion next to the load would wait for it.
+template <class S> using Raw = std::conditional_t<sizeof(S) == 4, float, unsigned short>;
+template <class S> __device__ __forceinline__ Raw<S> row_load(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff) {
     if constexpr (sizeof(S) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0));
-    else return (float)__builtin_bit_cast(S, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, 0));
+    else return (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, 0);
+}
+template <class S> __device__ __forceinline__ float value_of(Raw<S> x) {
+    if constexpr (sizeof(S) == 4) return x;
+    else return (float)__builtin_bit_cast(S, (unsigned short)x);
+}
+template <class S, int F> __device__ __forceinline__ void values_of(const Raw<S> (&x)[F], float (&v)[F]) {
+#pragma unroll
+    for (int i = 0; i < F; ++i) v[i] = value_of<S>(x[i]);
 }
 template <class S> __device__ __forceinline__ void row_store(float v, __amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff) {
     if constexpr (sizeof(S) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, voff, soff, 0);
@@ -173,7 +246,7 @@ template <class S, int F> struct LaneRows {
         for (int i = 0; i < F; ++i) v[i] = on ? (unsigned)(reverse ? TT - 1 - (F * sq + i) : F * sq + i) * st + (unsigned)(col * (int)sizeof(S)) : SC_OUT;
     }
     // the frames of a full tile, or of a tile whose frames from `left` on do not exist
-    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int sq, int left, float (&x)[F]) const {
+    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int sq, int left, Raw<S> (&x)[F]) const {
 #pragma unroll
         for (int i = 0; i < F; ++i) x[i] = row_load<S>(r, FULL || F * sq + i < left ? v[i] : SC_OUT, 0);
     }
@@ -193,14 +266,14 @@ template <class S, int TT, int NP> struct StateRows {
             v[k] = i < TT * NP && n < N ? ((unsigned)(reverse ? TT - 1 - m : m) * (unsigned)stride + (unsigned)n) * (unsigned)sizeof(S) : SC_OUT;
         }
     }
-    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int left, float (&x)[NB]) const {
+    template <bool FULL> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int left, Raw<S> (&x)[NB]) const {
 #pragma unroll
         for (int k = 0; k < NB; ++k) x[k] = row_load<S>(r, FULL || ((int)threadIdx.x + 256 * k) / NP < left ? v[k] : SC_OUT, 0);
     }
-    __device__ __forceinline__ void put(float* lds, const float (&x)[NB]) const {
+    __device__ __forceinline__ void put(float* lds, const Raw<S> (&x)[NB]) const {
 #pragma unroll
         for (int k = 0; k < NB; ++k)
-            if (TT * NP >= 256 || (int)threadIdx.x + 256 * k < TT * NP) lds[threadIdx.x + 256 * k] = x[k];
+            if (TT * NP >= 256 || (int)threadIdx.x + 256 * k < TT * NP) lds[threadIdx.x + 256 * k] = value_of<S>(x[k]);
     }
 };
 
@@ -234,7 +307,7 @@ template <int NS, bool C> struct ScanGroup {
 // grid (channel blocks, B, runs).  SUMMARY: leave this run's end state from zero and sum of D; otherwise the outputs.
 template <class S, int LN, int NS, bool SUMMARY>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
-    constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4;
+    constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4, W = lane_frames<LN>;
     using Rows = LaneRows<S, 4>;
     using BC = StateRows<S, TT, NP>;
     __shared__ __attribute__((aligned(16))) float sD[2][CB * LD], sU[2][CB * LD], sB[2][TT * NP], sC[2][SUMMARY ? 4 : TT * NP];
@@ -269,7 +342,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
     }
     arrived(h);
 
-    float ru[4], re[4], rz[4], rb[BC::NB], rc[BC::NB];            // the next tile's elements on their way
+    Raw<S> ru[4], re[4], rz[4], rb[BC::NB], rc[BC::NB];           // the next tile's elements on their way
     auto request = [&](auto full, int left) __attribute__((always_inline)) {
         ou.template load<full()>(rows_at(u), sq, left, ru);
         oe.template load<full()>(rows_at(e), sq, left, re);
@@ -294,17 +367,19 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
             for (int i = 0; i < 4; ++i) row_store<S>(0.f, rows_at(y), SC_OUT, 4 * i);
     }
     for (; t0 < stop; t0 += TT, buf ^= 1) {
-        float uc[4], gate[4], D4[4], U4[4];
-        steps_of<4>(a, re, bias, sq * 4, len - t0, D4);
+        float uc[4], gate[4], D4[4], U4[4], e4[4], z4[4];
+        values_of<S>(re, e4);
+        values_of<S>(ru, uc);
+        values_of<S>(rz, z4);
+        steps_of<4>(a, e4, bias, sq * 4, len - t0, D4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            U4[i] = D4[i] * ru[i];
-            uc[i] = ru[i];
+            U4[i] = D4[i] * uc[i];
             gate[i] = 1.f;
         }
         if (!SUMMARY && a.z)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) gate[i] = rz[i] * fast_sigmoid(rz[i]);
+            for (int i = 0; i < 4; ++i) gate[i] = z4[i] * fast_sigmoid(z4[i]);
         store_pack<float, 4>(&sD[buf][sch * LD + sq * 4], D4);
         store_pack<float, 4>(&sU[buf][sch * LD + sq * 4], U4);
         ob.put(sB[buf], rb);
@@ -340,10 +415,12 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
                 if (SUMMARY) dsum += at(g.D, i);
             }
             if constexpr (!SUMMARY) {
+                lanes_sum4<LN, 1>(y4);
+                float yw[W];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y4[i] = lanes_sum<LN>(y4[i]);
-                arrived(y4);
-                if (nq == 0) store_pack<float, 4>(rowD + 4 * q, y4);                     // the channel's lanes have read D there
+                for (int i = 0; i < W; ++i) yw[i] = y4[i];
+                arrived(yw);
+                if (nq % 4 == 0) store_pack<float, W>(rowD + 4 * q + nq / 4 * W, yw);      // the channel's lanes have read D there
             }
             if (q + 1 < TT / 4) g = next;
         }
@@ -353,8 +430,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
         load_pack<float, 4>(&sD[buf][sch * LD + sq * 4], o);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = fmaf(uc[i], skip, o[i]) * gate[i];
-        if (len - t0 >= TT) oy.template store<true>(rows_at(y), sq, TT, o);
-        else oy.template store<false>(rows_at(y), sq, len - t0, o);
+        oy.template store<false>(rows_at(y), sq, len - t0, o);
         y += adv * yt;
     }
     if (SUMMARY) {
@@ -400,7 +476,7 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) A2[j] = d < a.D && nq * NS + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
     arrived(A2);
-    float re[4], rz[4], rg[4], rc[BC::NB];
+    Raw<S> re[4], rz[4], rg[4], rc[BC::NB];
     auto request = [&](auto full, int left) __attribute__((always_inline)) {
         oe.template load<full()>(rows_at(e), sq, left, re);
         oz.template load<full()>(rows_at(z), sq, left, rz);
@@ -414,13 +490,14 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
     };
     if (t0 >= p0) fetch(len - t0);
     for (; t0 >= p0; t0 -= TT, buf ^= 1) {
-        float D4[4], G4[4];
-        steps_of<4>(a, re, bias, sq * 4, len - t0, D4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) G4[i] = rg[i];
+        float D4[4], G4[4], e4[4], z4[4];
+        values_of<S>(re, e4);
+        values_of<S>(rz, z4);
+        values_of<S>(rg, G4);
+        steps_of<4>(a, e4, bias, sq * 4, len - t0, D4);
         if (a.z)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) G4[i] *= rz[i] * fast_sigmoid(rz[i]);
+            for (int i = 0; i < 4; ++i) G4[i] *= z4[i] * fast_sigmoid(z4[i]);
         store_pack<float, 4>(&sD[buf][sch * LD + sq * 4], D4);
         store_pack<float, 4>(&sG[buf][sch * LD + sq * 4], G4);
         oc.put(sC[buf], rc);
@@ -491,7 +568,7 @@ template <int LN, int NS> struct ScanBwdLds {
 template <class S, int LN, int NS>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
     using L = ScanBwdLds<LN, NS>;
-    constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F;                  // F frames of a channel per thread and tile
+    constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F, W = lane_frames<LN>;                  // F frames of a channel per thread and tile
     constexpr int NP2 = TT * 2 * NP / 256;
     using Rows = LaneRows<S, F>;
     using BC = StateRows<S, TT, NP>;
@@ -553,7 +630,8 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         a.bc[(((long long)blk.x * a.T + max(stop, p0) + i / (2 * NP)) * a.B + b) * 2 * NP + i % (2 * NP)] = 0.f;
     arrived(r);
 
-    float ru[F], re[F], rz[F], rg[F], rb[BC::NB], rc[BC::NB], rh[NS];
+    Raw<S> ru[F], re[F], rz[F], rg[F], rb[BC::NB], rc[BC::NB];
+    float rh[NS];
     auto request = [&](auto full, int left) __attribute__((always_inline)) {
         ou.template load<full()>(rows_at(u), sq, left, ru);
         oe.template load<full()>(rows_at(e), sq, left, re);
@@ -576,13 +654,16 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         for (int i = 0; i < 3 * F + NP2; ++i) row_store<S>(0.f, rows_at(du), SC_OUT, 4 * i);       // (see scan_fwd_kernel)
     }
     for (; t0 >= p0; t0 -= TT) {
-        float D4[F], U4[F], S4[F], G4[F], Z4[F];
-        steps_of<F>(a, re, bias, sq * F, len - t0, D4);
+        float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F];
+        values_of<S>(ru, u4);
+        values_of<S>(re, e4);
+        values_of<S>(rz, z4);
+        values_of<S>(rg, G4);
+        steps_of<F>(a, e4, bias, sq * F, len - t0, D4);
 #pragma unroll
         for (int i = 0; i < F; ++i) {
-            S4[i] = fast_sigmoid(re[i] + bias);
-            U4[i] = D4[i] * ru[i];
-            G4[i] = rg[i];
+            S4[i] = fast_sigmoid(e4[i] + bias);
+            U4[i] = D4[i] * u4[i];
             Z4[i] = 0.f;
         }
         if (!a.softplus)
@@ -591,17 +672,17 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         if (a.z)
 #pragma unroll
             for (int i = 0; i < F; ++i) {
-                const float sg = fast_sigmoid(rz[i]);
-                G4[i] = rg[i] * (rz[i] * sg);
-                Z4[i] = rg[i] * (sg * fmaf(rz[i], 1.f - sg, 1.f));
+                const float sg = fast_sigmoid(z4[i]);
+                Z4[i] = G4[i] * (sg * fmaf(z4[i], 1.f - sg, 1.f));
+                G4[i] = G4[i] * (z4[i] * sg);
             }
 #pragma unroll
-        for (int i = 0; i < F; ++i) dskip = fmaf(G4[i], ru[i], dskip);
+        for (int i = 0; i < F; ++i) dskip = fmaf(G4[i], u4[i], dskip);
         store_pack<float, F>(sD + sch * LD + sq * F, D4);
         store_pack<float, F>(sU + sch * LD + sq * F, U4);
         store_pack<float, F>(sG + sch * LD + sq * F, G4);
         store_pack<float, F>(keep[0].v, D4);
-        store_pack<float, F>(keep[256].v, ru);
+        store_pack<float, F>(keep[256].v, u4);
         store_pack<float, F>(keep[512].v, S4);
         store_pack<float, F>(keep[768].v, G4);
         store_pack<float, F>(keep[1024].v, Z4);
@@ -641,7 +722,7 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
             gb.template load<NP>(rowD, rowU, sB, sC, k, nq);
             const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
             __builtin_amdgcn_sched_barrier(0);
-            float yo[4], bo[4], ko[4];
+            float o12[12];                                       // (k, b, y) of four frames
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
                 const int s = 4 * k + i;
@@ -650,9 +731,9 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
                     const float rj = fmaf(gb.Cv[i].v[j], gi, r[j]), hj = fmaf(dui, gb.B[i].v[j], q[s][j]), rq = rj * q[s][j];
-                    yo[i] = j ? fmaf(gb.Cv[i].v[j], hj, yo[i]) : gb.Cv[i].v[j] * hj;
-                    bo[i] = j ? fmaf(gb.B[i].v[j], rj, bo[i]) : gb.B[i].v[j] * rj;
-                    ko[i] = j ? fmaf(A[j], rq, ko[i]) : A[j] * rq;
+                    o12[2 + 3 * i] = j ? fmaf(gb.Cv[i].v[j], hj, o12[2 + 3 * i]) : gb.Cv[i].v[j] * hj;
+                    o12[1 + 3 * i] = j ? fmaf(gb.B[i].v[j], rj, o12[1 + 3 * i]) : gb.B[i].v[j] * rj;
+                    o12[0 + 3 * i] = j ? fmaf(A[j], rq, o12[0 + 3 * i]) : A[j] * rq;
                     dat[j] = fmaf(dt, rq, dat[j]);
                     vB[j] = rj * dui;
                     vC[j] = gi * hj;
@@ -663,19 +744,22 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
                 for (int j = 0; j < NS / 2; ++j) o[j] = v[j];
             }
+            lanes_sum4<LN, 3>(o12);
+            float ko[W], bo[W], yo[W];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                yo[i] = lanes_sum<LN>(yo[i]);
-                bo[i] = lanes_sum<LN>(bo[i]);
-                ko[i] = lanes_sum<LN>(ko[i]);
+            for (int i = 0; i < W; ++i) {
+                ko[i] = o12[3 * i];
+                bo[i] = o12[1 + 3 * i];
+                yo[i] = o12[2 + 3 * i];
             }
-            arrived(yo);
-            arrived(bo);
             arrived(ko);
-            if (nq == 0) {                                       // the channel's lanes have read these four frames
-                store_pack<float, 4>(rowD + 4 * k, ko);
-                store_pack<float, 4>(rowU + 4 * k, bo);
-                store_pack<float, 4>(rowG + 4 * k, yo);
+            arrived(bo);
+            arrived(yo);
+            if (nq % 4 == 0) {                                   // the channel's lanes have read these four frames
+                const int at_ = 4 * k + nq / 4 * W;
+                store_pack<float, W>(rowD + at_, ko);
+                store_pack<float, W>(rowU + at_, bo);
+                store_pack<float, W>(rowG + at_, yo);
             }
         }
 #pragma unroll
