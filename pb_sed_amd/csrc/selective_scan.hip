@@ -844,8 +844,9 @@ __global__ __launch_bounds__(SUM_THREADS) void scan_sum_kernel(const float* bc, 
 
 // ------------------------------------------------------------------------------------------------ one frame
 // u, delta, z [B][D] and b, c [B][N] at clip strides, state [B][D][N] float -> state_out (which may be the same memory).  Bound: HBM (the
-// states in and out).  LN lanes of four states share a channel; a block keeps the rates of its channels over `run` clips, and the next
-// clip's states are on their way while one is computed.  WHOLE: N is a multiple of four.
+// states in and out).  LN lanes of four states share a channel; a block keeps the rates of its channels over `run` clips, and everything
+// of the next clip is on its way while one is computed.  WHOLE: N is a multiple of four.  Measured: 384 clips x 1024 channels x 16
+// states, bfloat16: 11.2 us (55 MB, 4.9 TB/s; 16.3 with only the states under way early); one clip x 512 channels: 3.2 us (a launch).
 template <class S, int LN, bool WHOLE>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     constexpr int CB = 256 / LN, NS = 4;
@@ -860,25 +861,41 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
             if (has) load_loose<float, NS>(row + n0, v);
         } else load_states<NS>(row, n0, a.N, v);
     };
-    float A2[NS], h[NS], nxt[NS];
-    four(a.h0 + ((long long)b0 * a.D + d) * a.N, nxt);
+    struct Clip { S u, e, z; LoosePack<S, NS> B, C; float h[NS]; };        // raw: nothing waits for them before their turn
+    auto fetch = [&](int b) __attribute__((always_inline)) {
+        Clip f{};
+        f.u = static_cast<const S*>(a.u)[b * a.ub + d];
+        f.e = static_cast<const S*>(a.delta)[b * a.eb + d];
+        if (a.z) f.z = static_cast<const S*>(a.z)[b * a.zb + d];
+        const S *pb = static_cast<const S*>(a.b) + b * a.bb + n0, *pc = static_cast<const S*>(a.c) + b * a.cb + n0;
+        if constexpr (WHOLE) {
+            if (has) {
+                f.B = *reinterpret_cast<const LoosePack<S, NS>*>(pb);
+                f.C = *reinterpret_cast<const LoosePack<S, NS>*>(pc);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                if (n0 + j < a.N) { f.B.v[j] = pb[j]; f.C.v[j] = pc[j]; }
+        }
+        four(a.h0 + ((long long)b * a.D + d) * a.N, f.h);
+        return f;
+    };
+    Clip f, next = fetch(b0);
+    float A2[NS];
     four(a.a_log + (long long)d * a.N, A2);
 #pragma unroll
     for (int j = 0; j < NS; ++j) A2[j] = -LOG2E * rate_of(A2[j]);
     const float bias = a.dbias ? a.dbias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
     for (int b = b0; b < b1; ++b) {
-#pragma unroll
-        for (int j = 0; j < NS; ++j) h[j] = nxt[j];
-        if (b + 1 < b1) four(a.h0 + ((long long)(b + 1) * a.D + d) * a.N, nxt);
-        const float u = (float)static_cast<const S*>(a.u)[b * a.ub + d], z = a.z ? (float)static_cast<const S*>(a.z)[b * a.zb + d] : 0.f;
-        const float dt = step_of(a, (float)static_cast<const S*>(a.delta)[b * a.eb + d] + bias), du = dt * u;
-        float y = 0.f;
+        f = next;
+        if (b + 1 < b1) next = fetch(b + 1);
+        const float u = (float)f.u, z = (float)f.z, dt = step_of(a, (float)f.e + bias), du = dt * u;
+        float (&h)[NS] = f.h, y = 0.f;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-            const bool in = WHOLE ? has : n0 + j < a.N;
-            const float Bv = in ? (float)static_cast<const S*>(a.b)[b * a.bb + n0 + j] : 0.f, Cv = in ? (float)static_cast<const S*>(a.c)[b * a.cb + n0 + j] : 0.f;
-            h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], du * Bv);
-            y = fmaf(Cv, h[j], y);
+            h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], du * (float)f.B.v[j]);
+            y = fmaf((float)f.C.v[j], h[j], y);
         }
         y = lanes_sum<LN>(y);
         if (on) {
@@ -974,7 +991,7 @@ static int scan_bwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
 template <class S, int LN>
 static int scan_step_launch(ScanArgs& a, hipStream_t s) {
     const int blocks = (a.D + 256 / LN - 1) / (256 / LN);
-    // clips per block: as many as leave every CU eight blocks
+    // clips per block: as many as leave every CU eight blocks (384 x 1024 x 16: 11.2 us; one clip per block 14.5, four blocks per CU 11.6)
     const long long runs = (long long)blocks * a.B / (8ll * device_cus());
     a.run = runs < 1 ? 1 : runs > 64 ? 64 : (int)runs;
     const dim3 grid(blocks, (a.B + a.run - 1) / a.run);
