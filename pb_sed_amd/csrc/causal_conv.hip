@@ -24,6 +24,7 @@ struct CConvArgs {
 };
 
 constexpr int CC_G = 8, CC_BG = 4;              // positions per load group, forward and backward
+constexpr long long CC_BLOCKS = (1 << 24) - 1;  // of 256 threads: a launch has less than 2^32 of them
 
 template <class S, int V>
 __device__ __forceinline__ void zero_v(float (&v)[V]) {
@@ -317,6 +318,10 @@ static int cconv_launch(CConvArgs& a, int K, bool bwd, hipStream_t s) {
     const int full = 4, v = a.D >= full ? full : 1;
     a.ts = cconv_ts(a.T, a.B, a.D, v);
     a.nrun = (a.T + a.ts - 1) / a.ts;
+    if (!bwd && (long long)a.B * a.nrun * ((a.D + 64 * v - 1) / (64 * v)) > 4 * CC_BLOCKS) {
+        set_error("causal_conv_fwd: T = %d, B = %d, D = %d need more than %lld blocks", a.T, a.B, a.D, CC_BLOCKS);
+        return PBSED_E_UNSUPPORTED;
+    }
     if (v == 1) cconv_launch2<S, 1>(a, K, bwd, s);
     else cconv_launch2<S, 4>(a, K, bwd, s);
     return check_launch(bwd ? "causal_conv_bwd" : "causal_conv_fwd");
@@ -324,8 +329,8 @@ static int cconv_launch(CConvArgs& a, int K, bool bwd, hipStream_t s) {
 
 static int cconv_check(const char* name, int T, int B, int D, int K, int dtype) {
     if (dtype < 0 || dtype > 2) { set_error("%s: element type %d", name, dtype); return PBSED_E_ARG; }
-    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 24) || K < 2 || K > 8) {
-        set_error("%s: T = %d, B = %d, D = %d, K = %d (T <= 2^28, B <= 65535, D <= 2^24, 2 <= K <= 8)", name, T, B, D, K);
+    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 22) || K < 2 || K > 8) {
+        set_error("%s: T = %d, B = %d, D = %d, K = %d (T <= 2^28, B <= 65535, D <= 2^22, 2 <= K <= 8)", name, T, B, D, K);
         return PBSED_E_ARG;
     }
     return PBSED_OK;
@@ -393,8 +398,9 @@ extern "C" int pbsed_causal_conv_step(const void* x, const float* w, const float
                                       int D, int K, long long x_stride_b, int silu, int dtype, void* stream) {
     if (const int rc = cconv_check("causal_conv_step", 1, B, D, K, dtype)) return rc;
     if (!x || !w || !state || !state_out || !y) { set_error("causal_conv_step: null pointer"); return PBSED_E_ARG; }
-    const unsigned grid = (unsigned)(((long long)B * D + 255) / 256);
-    PBSED_ELEM(dtype, hipLaunchKernelGGL(causal_conv_step_kernel<S>, dim3(grid), dim3(256), 0, (hipStream_t)stream, static_cast<const S*>(x),
+    const long long grid = ((long long)B * D + 255) / 256;
+    if (grid > CC_BLOCKS) { set_error("causal_conv_step: B = %d, D = %d need more than %lld blocks", B, D, CC_BLOCKS); return PBSED_E_UNSUPPORTED; }
+    PBSED_ELEM(dtype, hipLaunchKernelGGL(causal_conv_step_kernel<S>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, static_cast<const S*>(x),
                                          x_stride_b, w, bias, static_cast<const S*>(state), static_cast<S*>(state_out), static_cast<S*>(y),
                                          B, D, K, silu));
     return check_launch("causal_conv_step");

@@ -312,8 +312,8 @@ static int norm_launch(const NormArgs& a, bool bwd, hipStream_t s) {
 
 static int norm_check(const char* name, long long rows, long long C, long long s0, long long s1, int dtype) {
     if (dtype < 0 || dtype > 2) { set_error("%s: element type %d", name, dtype); return PBSED_E_ARG; }
-    if (rows < 1 || rows > 0x3fffffff || C < 1 || C > 0x3fffffff || s0 < C || s1 < C) {
-        set_error("%s: %lld rows of %lld elements at strides %lld / %lld", name, rows, C, s0, s1);
+    if (rows < 1 || rows > 0x3fffffff || C < 1 || C > (1 << 24) || s0 < C || s1 < C) {
+        set_error("%s: %lld rows of %lld elements at strides %lld / %lld (at most 2^30 - 1 rows of 2^24)", name, rows, C, s0, s1);
         return PBSED_E_ARG;
     }
     return PBSED_OK;
@@ -334,7 +334,7 @@ extern "C" int pbsed_layer_norm_fwd(const void* x, const float* w, const float* 
 }
 
 extern "C" long long pbsed_layer_norm_workspace(long long rows, long long C) {
-    if (rows < 1 || rows > 0x3fffffff || C < 1 || C > 0x3fffffff) return 0;
+    if (rows < 1 || rows > 0x3fffffff || C < 1 || C > (1 << 24)) return 0;
     return (long long)norm_grid((int)rows, (int)C, true) * 2 * C;
 }
 

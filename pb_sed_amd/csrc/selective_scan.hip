@@ -952,8 +952,8 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
 
 static int scan_check(const char* name, int T, int B, int D, int N, int dtype) {
     if (dtype < 0 || dtype > 2) { set_error("%s: element type %d", name, dtype); return PBSED_E_ARG; }
-    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 24) || N < 1 || N > 64 || (long long)D * N > (1 << 30)) {
-        set_error("%s: T = %d, B = %d, D = %d, N = %d (T <= 2^28, B <= 65535, D <= 2^24, N <= 64)", name, T, B, D, N);
+    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 24) || N < 1 || N > 64 || (long long)D * (N + 2) >= (1 << 26)) {       // (64 parameter sums per 1024 threads, < 2^32 threads)
+        set_error("%s: T = %d, B = %d, D = %d, N = %d (T <= 2^28, B <= 65535, N <= 64, D (N + 2) < 2^26)", name, T, B, D, N);
         return PBSED_E_ARG;
     }
     return PBSED_OK;

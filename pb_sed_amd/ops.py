@@ -1436,6 +1436,15 @@ def _distinct(name, what, out, **inputs):
             _fail(name, f'{what} overlaps {key}')
 
 
+def _apart(name, **sums):
+    """Sums that a launch adds to (contiguous float32 or None) must not share memory with one another."""
+    used = [(v.data_ptr(), v.numel() * 4, what) for what, v in sums.items() if v is not None]
+    for i, (p, size, what) in enumerate(used):
+        for q, other, key in used[:i]:
+            if p < q + other and q < p + size:
+                _fail(name, f'{what} overlaps {key}')
+
+
 def _interleaved(a, b):
     """Disjoint channel ranges of one wider buffer: equal strides in front of the channels, multiples of the smallest of them, and the
     offset between the two modulo that leaves room for both rows."""
@@ -1492,6 +1501,7 @@ def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=
     pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
     ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
     pso = _like(name, 'dstate_out', dstate_out, (b, k - 1, d), x.dtype, dev, True)
+    _apart(name, dweight=dweight, dbias=dbias)
     if dx is None:
         dx = _empty(x, shape)
     else:
@@ -1599,6 +1609,7 @@ def selective_scan_bwd(dy, u, delta, a_log, b, c, saved, *, d=None, z=None, delt
     pda = _like(name, 'da_log', da_log, (width, n), f32, dev, True)
     pdd = _like(name, 'dd', dd, (width,), f32, dev, True)
     pdb = _like(name, 'ddelta_bias', ddelta_bias, (width,), f32, dev, True)
+    _apart(name, da_log=da_log, dd=dd, ddelta_bias=ddelta_bias)
     n_saved, n_ws = _scan_plan(dev, t, bs, width, n, True)
     psv = _have(name, 'saved', saved, (n_saved,), f32, dev, True)
     if dz is not None:
@@ -1686,6 +1697,7 @@ def layer_norm_bwd(dy, x, weight, stats, *, dweight=None, dbias=None):
     pst = _have(name, 'stats', stats, (rows, 2), torch.float32, dev, True)
     pdw = _like(name, 'dweight', dweight, (c,), torch.float32, dev, True)
     pdb = _like(name, 'dbias', dbias, (c,), torch.float32, dev, True)
+    _apart(name, dweight=dweight, dbias=dbias)
     dx = _empty(x, shape)
     floats = _floats('pbsed_layer_norm_workspace', dev, rows, c) if pdw or pdb else 0
     ws = x.new_empty(floats, dtype=torch.float32) if floats else None

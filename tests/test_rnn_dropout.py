@@ -152,3 +152,13 @@ def test_training_step_with_gru_dropout_on_the_gpu():
             losses.append(loss.item())
             assert all(torch.isfinite(p.grad).all() for p in model.parameters())
         assert losses[0] != losses[1]
+
+
+def test_first_pass_under_capture_is_refused(monkeypatch):
+    """The seed's copy from the host must not become a node of a graph."""
+    from pb_sed_amd import engine, modules
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    rnn = modules.build_rnn(8, 64, 2, 4, 16, dropout=.5)
+    with pytest.raises(RuntimeError, match='before a graph is captured'):
+        engine.dropout_state(rnn, torch.device('cuda', 0))
+    assert rnn.dropout_rng is None

@@ -469,6 +469,40 @@ def test_refusals(dev):
             raise AssertionError(f'call {i} was accepted')
 
 
+def test_sums_that_share_memory_are_refused(dev):
+    from pb_sed_amd import ops
+    f = lambda *s: torch.zeros(*s, device=dev)     # noqa: E731
+    x, w, a_log, bc, both = f(4, 2, 6), f(6, 3), f(6, 1), f(4, 2, 1), f(30)
+    saved = ops.selective_scan_fwd(x, x, a_log, bc, bc, save=True)[2]
+    stats = ops.layer_norm_fwd(x, save=True)[1]
+    for call in (lambda: ops.causal_conv_bwd(x, x, w, dweight=both[:18].view(6, 3), dbias=both[17:23]),
+                 lambda: ops.selective_scan_bwd(x, x, x, a_log, bc, bc, saved, da_log=both[:6].view(6, 1), dd=both[:6]),
+                 lambda: ops.selective_scan_bwd(x, x, x, a_log, bc, bc, saved, dd=both[:6], ddelta_bias=both[5:11]),
+                 lambda: ops.layer_norm_bwd(x, x, None, stats, dweight=both[:6], dbias=both[:6])):
+        with pytest.raises(ValueError, match='overlaps'):
+            call()
+    ops.layer_norm_bwd(x, x, None, stats, dweight=both[:6], dbias=both[6:12])
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """Sizes whose launch would have 2^32 threads or more in one dimension: refused before anything is launched (pointers never read)."""
+    from pb_sed_amd import _lib
+    lib = _lib.lib()
+    p = 1 << 20                                   # stands for any address
+    big = 1 << 22
+    strides = (ctypes.c_longlong * 16)()
+    calls = [
+        lambda: lib.pbsed_causal_conv_fwd(p, p, None, None, None, p, None, 1, 65535, big, 4, 65535 * big, big, 1, 0, 0, None),
+        lambda: lib.pbsed_causal_conv_step(p, p, None, p, p, p, 65535, big, 4, big, 1, 0, None),
+        lambda: lib.pbsed_causal_conv_step(p, p, None, p, p, p, 1, 2 * big, 4, 2 * big, 1, 0, None),
+        lambda: lib.pbsed_selective_scan_fwd(p, p, p, p, p, None, None, None, None, None, p, None, None, None, 0, strides, 1, 1, big, 16, 1, 0, 0, None),
+        lambda: lib.pbsed_layer_norm_fwd(p, None, None, p, None, 1, (1 << 24) + 1, (1 << 24) + 1, 1e-5, 0, None),
+    ]
+    for i, call in enumerate(calls):
+        assert call() < 0, i
+        assert lib.pbsed_last_error()
+
+
 def test_cpu_tensors_are_refused():
     from pb_sed_amd import ops
     x = torch.zeros(4, 2, 6)
