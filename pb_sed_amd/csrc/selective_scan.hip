@@ -237,6 +237,12 @@ template <int NS> __device__ __forceinline__ void arrived(float (&v)[NS]) {     
     for (int j = 0; j < NS; ++j) asm volatile("" : "+v"(v[j]));
 #endif
 }
+// What lanes of a wave leave in LDS for one another: the wave's LDS accesses keep their order, the compiler must too.
+__device__ __forceinline__ void wave_handover() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // offsets of a lane's F frames (F sq .. F sq + F-1 of a tile of TT) in column `col`, out of range where the lane has none
 template <class S, int F> struct LaneRows {
     unsigned v[F];
@@ -558,15 +564,21 @@ __device__ __forceinline__ void channel_sums(const float (&vB)[NS], const float 
 }
 
 // grid (channel blocks, B, runs).  Tiles of 16 frames from the back: the tile's states are recomputed from the saved state in front of
-// it and kept in registers (q_t = exp(D_t A) h_{t-1} and the exponential itself), then the adjoint runs back over them.  What a thread
-// needs again when the tile's sums are known (D, u, sigmoid(raw), g, dy silu'(z) of its four frames) waits in its own corner of LDS.
+// it and kept in registers beside the exponentials, then the adjoint runs back over them (r q = r exp(D A) h_{t-1} is the adjoint that
+// moves on times the state before).  What a thread
+// needs again when the tile's sums are known (D, u, sigmoid(raw), g, dy silu'(z) of its frames) waits in its own corner of LDS.  A wave
+// stages its own channels, so that a tile has one barrier (B, C and the sums over the block's channels).
+// Bound: vector instructions - some 45 per frame and wave (64 / LN channels) of which two are exponentials, a third of that again for
+// staging, and the longest clips' chains, behind whose ends the device runs empty.  Measured (500 frames x 32 clips of falling length x 512
+// channels x 16 states, float, under sustained load): forward 51 us, backward 118 us with its sums (whole sums in every lane 129).
 template <int LN, int NS> struct ScanBwdLds {
     static constexpr int NP = NS * LN, CB = 256 / LN, TT = SC_SAVE, LD = TT + 4, F = CB * TT / 256;
     static constexpr int rows = CB * LD, bc = TT * NP, part = 4 * TT * 2 * NP, keep = 5 * 256 * F;
-    static constexpr size_t bytes = (size_t)(3 * rows + 2 * bc + part + keep) * sizeof(float);
+    static constexpr int parts = NP <= 32 ? 2 : 1;               // buffers of the sums: with one, a tile ends with a second barrier
+    static constexpr size_t bytes = (size_t)(3 * rows + 4 * bc + parts * part + keep) * sizeof(float);
 };
 template <class S, int LN, int NS>
-__global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256, NS > 2 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
     using L = ScanBwdLds<LN, NS>;
     constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F, W = lane_frames<LN>;                  // F frames of a channel per thread and tile
     constexpr int NP2 = TT * 2 * NP / 256;
@@ -574,13 +586,14 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
     using BC = StateRows<S, TT, NP>;
     static_assert(F >= 1 && NP2 >= 1 && L::rows >= 256, "a tile has work for every thread");
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *sB = sG + L::rows, *sC = sB + L::bc, *sP = sC + L::bc;     // sP [4][TT][2 NP]
-    Pack<float, F>* keep = reinterpret_cast<Pack<float, F>*>(sP + L::part) + threadIdx.x;
+    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *lds_bc = sG + L::rows, *lds_part = lds_bc + 4 * L::bc;     // [2][B | C], [parts][4][TT][2 NP]
+    Pack<float, F>* keep = reinterpret_cast<Pack<float, F>*>(lds_part + L::parts * L::part) + threadIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
-    const int ch = wave * (64 / LN) + lane / LN;
+    constexpr int WC = 64 / LN;                                  // channels of a wave: it stages them for itself
+    const int ch = wave * WC + lane / LN;
     const ScanBlock blk = scan_block<S, CB>();
     const int b = blk.b, c = blk.c, d0 = blk.x * CB, d = d0 + ch;
-    const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;      // staging: channel, group of F frames
+    const int sch = wave * WC + lane % WC, sq = lane / WC, sd = d0 + sch;      // staging: channel, group of F frames
     const bool chan = sd < a.D, gated = a.z != nullptr;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
     const int p0 = c * a.run, p1 = min(p0 + a.run, a.T), stop = min(p1, len);
@@ -652,8 +665,12 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         fetch(len - t0);
 #pragma unroll
         for (int i = 0; i < 3 * F + NP2; ++i) row_store<S>(0.f, rows_at(du), SC_OUT, 4 * i);       // (see scan_fwd_kernel)
+        ob.put(lds_bc, rb);
+        oc.put(lds_bc + L::bc, rc);
     }
-    for (; t0 >= p0; t0 -= TT) {
+    __syncthreads();
+    for (int buf = 0; t0 >= p0; t0 -= TT, buf ^= 1) {
+        float *sB = lds_bc + buf * 2 * L::bc, *sC = sB + L::bc, *sP = lds_part + (L::parts > 1 ? buf * L::part : 0);
         float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F];
         values_of<S>(ru, u4);
         values_of<S>(re, e4);
@@ -686,15 +703,15 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         store_pack<float, F>(keep[512].v, S4);
         store_pack<float, F>(keep[768].v, G4);
         store_pack<float, F>(keep[1024].v, Z4);
-        ob.put(sB, rb);
-        oc.put(sC, rc);
         float h[NS];
 #pragma unroll
         for (int j = 0; j < NS; ++j) h[j] = rh[j];
-        __syncthreads();
+        wave_handover();
         if (t0 - TT >= p0) fetch(len - t0 + TT);
         float *rowD = sD + ch * LD, *rowU = sU + ch * LD, *rowG = sG + ch * LD;
-        float ex[TT][NS], q[TT][NS];
+        float ex[TT][NS], hs[TT][NS], h0[NS];                    // hs[t]: the state behind frame t
+#pragma unroll
+        for (int j = 0; j < NS; ++j) h0[j] = h[j];
         ScanGroup<NS, false> gr;
         gr.template load<NP>(rowD, rowU, sB, nullptr, 0, nq);
 #pragma unroll
@@ -710,8 +727,8 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
-                    q[4 * k + i][j] = ex[4 * k + i][j] * h[j];
-                    h[j] = fmaf(at(gr.U, i), gr.B[i].v[j], q[4 * k + i][j]);
+                    h[j] = fmaf(ex[4 * k + i][j], h[j], at(gr.U, i) * gr.B[i].v[j]);
+                    hs[4 * k + i][j] = h[j];
                 }
             if (k + 1 < TT / 4) gr = next;
         }
@@ -730,14 +747,15 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
                 float vB[NS], vC[NS], v[NS / 2];
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
-                    const float rj = fmaf(gb.Cv[i].v[j], gi, r[j]), hj = fmaf(dui, gb.B[i].v[j], q[s][j]), rq = rj * q[s][j];
+                    const float rj = fmaf(gb.Cv[i].v[j], gi, r[j]), hj = hs[s][j];
+                    r[j] = rj * ex[s][j];
+                    const float rq = r[j] * (s ? hs[s ? s - 1 : 0][j] : h0[j]);
                     o12[2 + 3 * i] = j ? fmaf(gb.Cv[i].v[j], hj, o12[2 + 3 * i]) : gb.Cv[i].v[j] * hj;
                     o12[1 + 3 * i] = j ? fmaf(gb.B[i].v[j], rj, o12[1 + 3 * i]) : gb.B[i].v[j] * rj;
                     o12[0 + 3 * i] = j ? fmaf(A[j], rq, o12[0 + 3 * i]) : A[j] * rq;
                     dat[j] = fmaf(dt, rq, dat[j]);
                     vB[j] = rj * dui;
                     vC[j] = gi * hj;
-                    r[j] = rj * ex[s][j];
                 }
                 channel_sums<LN, NS>(vB, vC, v);
                 float* o = sP + (wave * TT + s) * 2 * NP + (lane >> 5) * NP + nq * NS + ((lane >> 4) & 1) * (NS / 2);
@@ -764,6 +782,10 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (sums over a tile first: long clips keep their digits)
+        if (t0 - TT >= p0) {                                     // B and C are the block's: the next tile's go where the last one's were
+            ob.put(lds_bc + (buf ^ 1) * 2 * L::bc, rb);
+            oc.put(lds_bc + (buf ^ 1) * 2 * L::bc + L::bc, rc);
+        }
         __syncthreads();
         const Pack<float, F> kk = *reinterpret_cast<const Pack<float, F>*>(sD + sch * LD + sq * F), bb = *reinterpret_cast<const Pack<float, F>*>(sU + sch * LD + sq * F);
         const Pack<float, F> yy = *reinterpret_cast<const Pack<float, F>*>(sG + sch * LD + sq * F);
@@ -793,7 +815,7 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
         if (len - t0 >= TT) write(std::true_type(), TT);
         else write(std::false_type(), len - t0);
         du += adv * row; de += adv * row; dz += adv * a.dzt; bc += adv * a.B * 2 * NP;
-        __syncthreads();                                         // before the next tile is staged
+        if (L::parts == 1) __syncthreads();
     }
     if (a.dh0 && d < a.D && c == 0) store_states<NS>(a.dh0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
     if (!a.sums) return;
@@ -804,14 +826,15 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(ScanArgs a) {
             if (nq * NS + j < a.N) out[(long long)d * a.N + nq * NS + j] = A[j] * da[j];
     }
     // the groups of frames of a channel meet in LDS
-    sD[tid] = dskip;
-    sU[tid] = dbias;
     __syncthreads();
-    if (tid < CB && chan) {
+    sD[sq * CB + sch] = dskip;
+    sU[sq * CB + sch] = dbias;
+    __syncthreads();
+    if (tid < CB && d0 + tid < a.D) {
         float s0 = sD[tid], s1 = sU[tid];
         for (int k = 1; k < 256 / CB; ++k) { s0 += sD[tid + k * CB]; s1 += sU[tid + k * CB]; }
-        out[(long long)a.D * a.N + sd] = s0;
-        out[(long long)a.D * (a.N + 1) + sd] = s1;
+        out[(long long)a.D * a.N + d0 + tid] = s0;
+        out[(long long)a.D * (a.N + 1) + d0 + tid] = s1;
     }
 }
 
@@ -920,8 +943,9 @@ struct ScanPlan {
 // Frames are cut into runs where channel blocks x clips leave CUs with hardly more than one block: a lone block per CU is bound by the
 // latency of its chain, and a cut costs the first launch (about 0.7 of the main one's work).  Up to SC_FOLD runs the main launch folds
 // those in front of its own by itself; more are folded by scan_runs_kernel, whose cost grows with the channels.  Measured (forward,
-// backward us): 192 blocks, T 1001, bf16: 83, 233 uncut; 64, 135 in 4 runs; 62, 127 in 5; 63, 135 in 8; 98, 173 in 32.  512 blocks, T 500,
-// float: 51, 148 uncut; 67, 148 in 2.  16 blocks, T 40000: 357 in 16; 205 in 64; 193 in 128; 192 in 250.  20 blocks, T 313: 34 uncut, 20 in 7.
+// backward us, N = 16): 192 blocks, T 1001, bfloat16: 72, 191 uncut; 60, 120 in 4 runs; 58, 113 in 5; 60, 121 in 8.  512 blocks, T 500,
+// float: 49, 132 uncut; 65, 137 in 2.  16 blocks, T 40000, bfloat16: 357 in 16; 205 in 64; 193 in 128; 192 in 250 (with the first form
+// of the lane sums).  20 blocks, T 313: 34 uncut, 20 in 7.
 constexpr int SC_FOLD = 16;
 static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     ScanPlan p{};
