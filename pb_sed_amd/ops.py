@@ -1340,13 +1340,21 @@ def _fail(name, message):
 
 def _elem(name, x, dim):
     """Element-type code and device of the operator's leading tensor [..., channels] with ``dim`` axes (0: any)."""
-    _lib.require_gpu(x)
+    if not x.is_cuda:
+        _lib.require_gpu(x)
     code = DTYPE_CODES.get(x.dtype)
     if code is None:
         _fail(name, f'element type {x.dtype}; float32, bfloat16 or float16')
     if (dim and x.dim() != dim) or not x.dim() or not x.numel():
         _fail(name, f'expected a {dim or "1 or more"}-d tensor that is not empty, got {tuple(x.shape)}')
     return code, x.get_device()
+
+
+def _lead(name, what, x):
+    """Address of the leading tensor: unit stride over its channels."""
+    if x.shape[-1] != 1 and x.stride(-1) != 1:
+        _fail(name, f'{what} needs unit stride over its channels')
+    return x.data_ptr()
 
 
 def _like(name, what, v, shape, dtype, dev, whole=False):
@@ -1436,12 +1444,11 @@ def _distinct(name, what, out, **inputs):
             _fail(name, f'{what} overlaps {key}')
 
 
-def _apart(name, **sums):
-    """Sums that a launch adds to (contiguous float32 or None) must not share memory with one another."""
-    used = [(v.data_ptr(), v.numel() * 4, what) for what, v in sums.items() if v is not None]
-    for i, (p, size, what) in enumerate(used):
-        for q, other, key in used[:i]:
-            if p < q + other and q < p + size:
+def _apart(name, *sums):
+    """Sums that a launch adds to must not share memory: (what, address or None, floats) each."""
+    for i, (what, p, n) in enumerate(sums):
+        for key, q, m in sums[:i]:
+            if p and q and p < q + 4 * m and q < p + 4 * n:
                 _fail(name, f'{what} overlaps {key}')
 
 
@@ -1472,7 +1479,7 @@ def causal_conv_fwd(x, weight, bias=None, *, silu=True, seq_len=None, reverse=Fa
     name = 'causal_conv_fwd'
     code, dev = _elem(name, x, 3)
     t, b, d = shape = x.shape
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     pw, k = _conv_weight(name, weight, d, dev)
     pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
     pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
@@ -1492,7 +1499,7 @@ def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=
     name = 'causal_conv_bwd'
     code, dev = _elem(name, x, 3)
     t, b, d = shape = x.shape
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     pg = _have(name, 'dy', dy, shape, x.dtype, dev)
     pw, k = _conv_weight(name, weight, d, dev)
     pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
@@ -1501,7 +1508,7 @@ def causal_conv_bwd(dy, x, weight, bias=None, *, dweight=None, dbias=None, silu=
     pl = _like(name, 'seq_len', seq_len, (b,), torch.int32, dev, True)
     ps = _like(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
     pso = _like(name, 'dstate_out', dstate_out, (b, k - 1, d), x.dtype, dev, True)
-    _apart(name, dweight=dweight, dbias=dbias)
+    _apart(name, ('dweight', pdw, d * k), ('dbias', pdb, d))
     if dx is None:
         dx = _empty(x, shape)
     else:
@@ -1533,7 +1540,7 @@ def causal_conv_step(x, weight, bias, state, *, silu=True, state_out=None):
     name = 'causal_conv_step'
     code, dev = _elem(name, x, 2)
     b, d = shape = x.shape
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     pw, k = _conv_weight(name, weight, d, dev)
     pb = _like(name, 'bias', bias, (d,), torch.float32, dev, True)
     ps = _have(name, 'state', state, (b, k - 1, d), x.dtype, dev, True)
@@ -1551,7 +1558,7 @@ def _scan_operands(name, dim, u, delta, a_log, b, c, d, z, delta_bias):
         _fail(name, f'a_log must be [D, N] with 1 <= N <= 64, got {tuple(a_log.shape)}')
     width, n = shape[-1], a_log.shape[1]
     states = (*shape[:-1], n)
-    return code, dev, n, (_like(name, 'u', u, shape, dt, dev), _have(name, 'delta', delta, shape, dt, dev),
+    return code, dev, n, (_lead(name, 'u', u), _have(name, 'delta', delta, shape, dt, dev),
                           _have(name, 'a_log', a_log, (width, n), f32, dev, True), _have(name, 'b', b, states, dt, dev),
                           _have(name, 'c', c, states, dt, dev), _like(name, 'd', d, (width,), f32, dev, True),
                           _like(name, 'z', z, shape, dt, dev), _like(name, 'delta_bias', delta_bias, (width,), f32, dev, True))
@@ -1609,7 +1616,7 @@ def selective_scan_bwd(dy, u, delta, a_log, b, c, saved, *, d=None, z=None, delt
     pda = _like(name, 'da_log', da_log, (width, n), f32, dev, True)
     pdd = _like(name, 'dd', dd, (width,), f32, dev, True)
     pdb = _like(name, 'ddelta_bias', ddelta_bias, (width,), f32, dev, True)
-    _apart(name, da_log=da_log, dd=dd, ddelta_bias=ddelta_bias)
+    _apart(name, ('da_log', pda, width * n), ('dd', pdd, width), ('ddelta_bias', pdb, width))
     n_saved, n_ws = _scan_plan(dev, t, bs, width, n, True)
     psv = _have(name, 'saved', saved, (n_saved,), f32, dev, True)
     if dz is not None:
@@ -1672,7 +1679,7 @@ def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5, save=False):
     shape = x.shape
     c = shape[-1]
     rows = x.numel() // c
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     xs = _row_stride(name, 'x', x)
     pw = _like(name, 'weight', weight, (c,), torch.float32, dev, True)
     pb = _like(name, 'bias', bias, (c,), torch.float32, dev, True)
@@ -1691,13 +1698,13 @@ def layer_norm_bwd(dy, x, weight, stats, *, dweight=None, dbias=None):
     shape = x.shape
     c = shape[-1]
     rows = x.numel() // c
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     pg = _have(name, 'dy', dy, shape, x.dtype, dev)
     pw = _like(name, 'weight', weight, (c,), torch.float32, dev, True)
     pst = _have(name, 'stats', stats, (rows, 2), torch.float32, dev, True)
     pdw = _like(name, 'dweight', dweight, (c,), torch.float32, dev, True)
     pdb = _like(name, 'dbias', dbias, (c,), torch.float32, dev, True)
-    _apart(name, dweight=dweight, dbias=dbias)
+    _apart(name, ('dweight', pdw, c), ('dbias', pdb, c))
     dx = _empty(x, shape)
     floats = _floats('pbsed_layer_norm_workspace', dev, rows, c) if pdw or pdb else 0
     ws = x.new_empty(floats, dtype=torch.float32) if floats else None
@@ -1719,7 +1726,7 @@ def dropout(x, p, rng, *, site=0, residual=None, out=None):
         _fail(name, f'p = {p} is not in [0, 1]')
     if not 0 <= site < 1 << 31:
         _fail(name, f'site = {site}')
-    px = _like(name, 'x', x, shape, x.dtype, dev)
+    px = _lead(name, 'x', x)
     pr = _have(name, 'rng', rng, (2,), torch.int64, dev, True)
     pres = _like(name, 'residual', residual, shape, x.dtype, dev)
     if out is None:
