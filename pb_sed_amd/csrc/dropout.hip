@@ -8,7 +8,8 @@
 // there do not survive.
 //
 // Bound: HBM (reads + one write); seven rounds are 14 32 x 32 -> 64 multiplications per four elements, which stay below the memory
-// time.
+// time.  Measured: 65536 rows of 1000 bfloat16 without residual: 51 us (5.1 TB/s; a large copy reaches 4.67); 16000 rows of 256 float,
+// with residual and without: 8 us on average (16 MB a tensor, in the caches).
 #include "elem.h"
 #include "pbsed_internal.h"
 

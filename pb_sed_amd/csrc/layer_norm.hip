@@ -7,7 +7,9 @@
 // backward pass their column sums of dy xh and dy - in registers; the sums leave as one row of partials per block, which a second
 // launch adds in a fixed order (no atomics: results are reproducible).
 //
-// Bound: HBM (forward x in, y out; backward x and dy in, dx out).
+// Bound: HBM (forward x in, y out; backward x and dy in, dx out).  Measured: 20011 rows of 1023 bfloat16: forward 18 us (4.6 TB/s, a large
+// copy reaches 4.67), backward 25 us (4.8 TB/s), its weights' sums 4 us; with element loads for the odd width 58 and 75.  16000 rows of
+// 256 float (16 MB a tensor, in the caches): 8, 10 and 3 us.
 #include "elem.h"
 #include "pbsed_internal.h"
 
@@ -259,7 +261,10 @@ __global__ __launch_bounds__(SUM_THREADS) void norm_sum_kernel(const float* ws, 
     sum_partials(ws, P, W, sg, blockIdx.x * 16, red);
 }
 
-// lanes per row and elements per lane
+// lanes per row and elements per lane: 16 lanes where a row has no more than 64 columns, a wave up to 2048 (row sums are lane exchanges,
+// without a barrier), a block above.  Measured on 16000 rows (forward, backward us): 64 float columns 3.7, 9.5 with 16 lanes, 5.2, 9.3
+// with 64; 256: 6.8, 15.2 with 16, 6.7, 12.4 with 64, 13.2, 20.5 with 256; 2048 bfloat16: 22.6, 33.2 with 64, 21.7, 38.9 with 256 (float:
+// 42.6, 49.5 and 41.9, 57.1).
 static void norm_shape(int C, int* lpr, int* e) {
     if (C <= 64) { *lpr = 16; *e = 4; }
     else if (C <= 1024) { *lpr = 64; *e = C <= 256 ? 4 : C <= 512 ? 8 : 16; }
