@@ -763,7 +763,7 @@ def gru_flags_raise(host_words):
             raise RuntimeError('persistent GRU scan: a workgroup of an XCD-local ring was dispatched to another XCD than the '
                                'placement probe observed (partition mode / CU mask changed?); this step\'s results were '
                                'discarded (the optimiser update was skipped on the device) and the XCD-local exchange is '
-                               'now off for this process (PBSED_GRU_XCD_LOCAL=0 does the same from the start).')
+                               'now off for this process (it is off from the start without PBSED_GRU_XCD_LOCAL=1).')
         raise RuntimeError('persistent GRU scan: inter-workgroup hand-off timed out; this step\'s results were discarded '
                            '(the optimiser update was skipped on the device).  PBSED_GRU_PERSIST=0 selects the '
                            'launch-per-step scans.')
