@@ -9,8 +9,7 @@ mkdir -p build
 pids=()
 for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm causal_conv selective_scan layer_norm dropout misc logmel postproc collective; do
   if [ ! -f build/$f.o ] || [ -n "$(find $f.hip build.sh *.h *.inc -newer build/$f.o)" ]; then
-    # logmel: products and sums contract within a statement only, which leaves the transform's roundings close to those of the packed
-    # instructions (across statements the fine-tuning step's max-pool decisions move by a rounding)
+    # logmel: products and sums contract within a statement only; the transform's fused multiply-adds are written out (fft512.h)
     EXTRA=""; [ $f = logmel ] && EXTRA="-ffp-contract=on"
     $HIPCC $FLAGS $EXTRA -c $f.hip -o build/$f.o &
     pids+=($!)

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void logmel_kernel(LogmelArgs a) {
             const cpx d = cpx{zk.x - zr.x, zk.y + zr.y};
             const cpx o = cpx{.5f * d.y, -.5f * d.x};
             const cpx xk = cadd(e, cmul(twp[r], o));
-            Prow[lane + 64 * r] = xk.x * xk.x + xk.y * xk.y;
+            Prow[lane + 64 * r] = fmaf(xk.x, xk.x, xk.y * xk.y);
         }
         if (lane == 0) { const float n = v[0].x - v[0].y; Prow[512] = n * n; }
         else if (lane < 4) Prow[512 + lane] = 0.f;
