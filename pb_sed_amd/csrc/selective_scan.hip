@@ -577,8 +577,10 @@ template <int LN, int NS> struct ScanBwdLds {
     static constexpr int parts = NP <= 32 ? 2 : 1;               // buffers of the sums: with one, a tile ends with a second barrier
     static constexpr size_t bytes = (size_t)(3 * rows + 4 * bc + parts * part + keep) * sizeof(float);
 };
+// (three blocks per CU: 168 registers, which four lanes per channel and four states per lane overrun - N = 8: forward and backward of
+// 500 x 32 x 512 float 204 us with three, 170 with two)
 template <class S, int LN, int NS>
-__global__ __launch_bounds__(256, NS > 2 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
     using L = ScanBwdLds<LN, NS>;
     constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F, W = lane_frames<LN>;                  // F frames of a channel per thread and tile
     constexpr int NP2 = TT * 2 * NP / 256;
@@ -945,7 +947,7 @@ struct ScanPlan {
 // those in front of its own by itself; more are folded by scan_runs_kernel, whose cost grows with the channels.  Measured (forward,
 // backward us, N = 16): 192 blocks, T 1001, bfloat16: 72, 191 uncut; 60, 120 in 4 runs; 58, 113 in 5; 60, 121 in 8.  512 blocks, T 500,
 // float: 49, 132 uncut; 65, 137 in 2.  16 blocks, T 40000, bfloat16: 357 in 16; 205 in 64; 193 in 128; 192 in 250 (with the first form
-// of the lane sums).  20 blocks, T 313: 34 uncut, 20 in 7.
+// of the lane sums).  20 blocks, T 313: 34 uncut, 20 in 7.  44 blocks (N = 8), T 2000: 46, 98 in 16; 54, 108 in 32; 53, 112 in 64.
 constexpr int SC_FOLD = 16;
 static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     ScanPlan p{};
@@ -959,7 +961,7 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     p.run = (T + grain - 1) / grain * grain;
     if (have * 8 <= cus * 9) {
         long long runs = 4 * cus / have;
-        if (runs > SC_FOLD) runs = 8 * cus / have;
+        if (runs > SC_FOLD) runs = SC_FOLD * have >= 5 * cus / 2 ? SC_FOLD : 8 * cus / have;
         if (runs > 256) runs = 256;
         const int len = (int)(((T + runs - 1) / runs + grain - 1) / grain * grain);
         p.run = len > least ? len : least;
