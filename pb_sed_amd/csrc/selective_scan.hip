@@ -947,7 +947,8 @@ struct ScanPlan {
 // those in front of its own by itself; more are folded by scan_runs_kernel, whose cost grows with the channels.  Measured (forward,
 // backward us, N = 16): 192 blocks, T 1001, bfloat16: 72, 191 uncut; 60, 120 in 4 runs; 58, 113 in 5; 60, 121 in 8.  512 blocks, T 500,
 // float: 49, 132 uncut; 65, 137 in 2.  16 blocks, T 40000, bfloat16: 357 in 16; 205 in 64; 193 in 128; 192 in 250 (with the first form
-// of the lane sums).  20 blocks, T 313: 34 uncut, 20 in 7.  44 blocks (N = 8), T 2000: 46, 98 in 16; 54, 108 in 32; 53, 112 in 64.
+// of the lane sums).  20 blocks, T 313: 34 uncut, 20 in 7.  44 blocks (N = 8), T 2000: 46, 98 in 16; 54, 108 in 32; 53, 112 in 64.  Short
+// ones are not cut (2 x 128 channels, N = 8: 8.7, 20.8 uncut and 11.9, 22.3 in runs at 64 frames, 14.5, 33.7 and 12.5, 23.2 at 128).
 constexpr int SC_FOLD = 16;
 static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     ScanPlan p{};
@@ -959,7 +960,7 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     const long long have = (long long)p.blocks * B, cus = device_cus();
     const int grain = p.cb >= 64 ? 16 : 1024 / p.cb, least = grain < 24 ? 48 : 2 * grain;     // a run is a number of (forward) tiles
     p.run = (T + grain - 1) / grain * grain;
-    if (have * 8 <= cus * 9) {
+    if (have * 8 <= cus * 9 && T >= 128) {
         long long runs = 4 * cus / have;
         if (runs > SC_FOLD) runs = SC_FOLD * have >= 5 * cus / 2 ? SC_FOLD : 8 * cus / have;
         if (runs > 256) runs = 256;
