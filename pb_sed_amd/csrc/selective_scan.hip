@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
         g.template load<NP>(rowD, rowU, sB[buf], sC[buf], 0, nq);
 #pragma unroll
         for (int q = 0; q < TT / 4; ++q) {
-            if (!SUMMARY && 4 * q % SC_SAVE == 0 && a.saved && (TT >= SC_SAVE || t0 % SC_SAVE == 0) && d < a.D && (q == 0 || t0 + 4 * q < a.T))
+            if (!SUMMARY && 4 * q % SC_SAVE == 0 && a.saved && d < a.D && (q == 0 || t0 + 4 * q < a.T))
                 store_pack<float, NS>(a.saved + (((long long)((t0 + 4 * q) / SC_SAVE) * a.B + b) * a.D + d) * NP + nq * NS, h);
             ScanGroup<NS, !SUMMARY> next;
             if (q + 1 < TT / 4) next.template load<NP>(rowD, rowU, sB[buf], sC[buf], q + 1, nq);
@@ -958,7 +958,7 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     p.cb = 256 / p.ln;
     p.blocks = (D + p.cb - 1) / p.cb;
     const long long have = (long long)p.blocks * B, cus = device_cus();
-    const int grain = p.cb >= 64 ? 16 : 1024 / p.cb, least = grain < 24 ? 48 : 2 * grain;     // a run is a number of (forward) tiles
+    const int grain = 1024 / p.cb, least = grain < 24 ? 48 : 2 * grain;                       // a run is a number of (forward) tiles
     p.run = (T + grain - 1) / grain * grain;
     if (have * 8 <= cus * 9 && T >= 128) {
         long long runs = 4 * cus / have;

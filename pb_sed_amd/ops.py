@@ -1361,21 +1361,21 @@ def _like(name, what, v, shape, dtype, dev, whole=False):
     """Checks an operand: shape, type, device; unit stride over its channels (``whole``: contiguous).  Returns its address (None: NULL)."""
     if v is None:
         return None
-    if not isinstance(v, torch.Tensor) or v.shape != shape or v.dtype != dtype or v.get_device() != dev:
-        _fail(name, f'{what} must be a {dtype} tensor of shape {tuple(shape)} on device {dev}, got '
-                    + (f'{v.dtype} {tuple(v.shape)} on {v.device}' if isinstance(v, torch.Tensor) else repr(type(v))))
+    if not isinstance(v, torch.Tensor):
+        _fail(name, f'{what} must be a {dtype} tensor of shape {tuple(shape)} on device {dev}, got {type(v)!r}')
+    if v.shape == shape and v.dtype is dtype and v.get_device() == dev and (v.is_contiguous() or not whole and v.stride(-1) == 1):
+        return v.data_ptr()
+    if v.shape != shape or v.dtype != dtype or v.get_device() != dev:
+        _fail(name, f'{what} must be a {dtype} tensor of shape {tuple(shape)} on device {dev}, got {v.dtype} {tuple(v.shape)} on {v.device}')
     if whole:
-        if not v.is_contiguous():
-            _fail(name, f'{what} must be contiguous')
-    elif shape[-1] != 1 and v.stride(-1) != 1:
+        _fail(name, f'{what} must be contiguous')
+    if shape[-1] != 1:
         _fail(name, f'{what} needs unit stride over its channels')
     return v.data_ptr()
 
 
-def _have(name, what, v, *args):
-    if v is None:
-        _fail(name, f'{what} is missing')
-    return _like(name, what, v, *args)
+def _have(name, what, v, shape, dtype, dev, whole=False):
+    return _like(name, what, v, shape, dtype, dev, whole) or _fail(name, f'{what} is missing')
 
 
 def _launch(dev, entry, *args):
