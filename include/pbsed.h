@@ -433,11 +433,13 @@ int pbsed_event_frames(const float* scores, const float* thr, const int* len, in
                        int max_events, void* stream);
 
 /* ---- state-space sequence layers (the recurrent part of pb_sed/models/weak_label/crnn.py:61-67 as a selective scan instead of a
- * GRU; padertorch has no such layer - new in the build).  Activations are time-major [T][B][channels] in one of three element types
+ * GRU; padertorch has no such layer).  Activations are time-major [T][B][channels] in one of three element types
  * (`dtype`), unit stride over channels, strides over frames and clips in elements; parameters, states and parameter gradients are
  * float.  seq_len [B] or NULL (= T): frames behind it are not read and their outputs are 0; `reverse` != 0 scans a clip's valid
  * frames from the last to the first.  Parameter gradients are ADDED to their buffers (any may be NULL), in a fixed order: results
- * are reproducible.  Workspaces are the caller's, used only by the launches of the call. */
+ * are reproducible.  Workspaces are the caller's, used only by the launches of the call.  Limits (an error code and a message beyond
+ * them): T <= 2^28, B <= 65535; convolution D <= 2^22; scan N <= 64, D (N + 2) < 2^26, frame strides < 2^23; layer norm rows < 2^30 of at
+ * most 2^24 elements; fewer than 2^32 threads in a launch's dimension. */
 #define PBSED_F32 0
 #define PBSED_BF16 1
 #define PBSED_F16 2
