@@ -643,6 +643,38 @@ def test_captured_layer_replays_with_new_masks_and_inputs():
 
 
 @pytest.mark.gpu
+def test_captured_frames_move_the_states_on():
+    """The one-frame forms captured into a graph, states in place: replays on new inputs equal the eager calls, with eager work between."""
+    from pb_sed_amd import ops
+    dev = 'cuda:0'
+    g = torch.Generator().manual_seed(5)
+    b, d, n = 5, 70, 12
+    p = layer_parameters(g, d, n, dev)
+    x, bc = normal(g, b, d).float().to(dev), normal(g, b, 2 * n).float().to(dev)
+
+    def frame(conv_state, state):
+        u = ops.causal_conv_step(x, p['cw'], p['cb'], conv_state)
+        return ops.selective_scan_step(u, x, p['a_log'], bc[:, :n], bc[:, n:], state, d=p['d'], z=x, delta_bias=p['db'])
+    states = [torch.zeros(b, 3, d, device=dev), torch.zeros(b, d, n, device=dev)]
+    own = [v.clone() for v in states]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        frame(*[v.clone() for v in states])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = frame(*states)
+    for i in range(5):
+        x.copy_(normal(torch.Generator().manual_seed(10 + i), b, d))
+        want = frame(*own)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and all(torch.equal(u, v) for u, v in zip(states, own)), i
+    assert float(states[1].abs().max()) > 0
+
+
+@pytest.mark.gpu
 def test_two_streams_and_repeated_calls_agree():
     """Calls on two streams at once (workspaces are per call) and repeated calls give the same bits."""
     from pb_sed_amd import ops
