@@ -35,7 +35,7 @@ struct ScanArgs {
     float* sums;                                       // backward: [B nrun][D N + 2 D] partial sums of da_log | dskip | ddelta_bias
     long long ut, ub, et, eb, bt, bb, ct, cb, zt, zb, gt, gb, dzt, dzb;      // strides over frames and clips (elements)
     int T, B, D, N, reverse, softplus, nrun, run;      // run: frames per run, a number of tiles
-    int folded;                                        // runs hold the states in front of the runs (scan_runs_kernel has been there)
+    int folded;                                        // runs hold the states in front of the runs (a scan_runs kernel has been there)
 };
 
 constexpr float LOG2E = 1.44269504088896341f;
@@ -165,7 +165,7 @@ __device__ __forceinline__ void fold_runs(const ScanArgs& a, int c, int from, in
         for (int j = 0; j < NS; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], s[j]);
     }
 }
-// Many runs (up to 256): their end states become the states in front of them, in place.  A lane owns one state; wave w of a block's 16
+// Many runs (up to 256) of steps that softplus made (factors up to one): their end states become the states in front of them, in place.  A lane owns one state; wave w of a block's 16
 // takes runs 16 w .. 16 w + 15 of the order, holds them in registers, and learns through LDS what the waves in front of it add up to.
 // back: from the last run to the first, starting from dh_out.
 __global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int back) {
@@ -201,6 +201,67 @@ __global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int
         const int k = wave * 16 + i, c = back ? a.nrun - 1 - k : k;
         if (on && k < a.nrun) a.runs[(long long)c * M + m] = x;
         x = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2), x, s[i]);
+    }
+}
+
+// Steps below zero (softplus = 0 only) have factors above one, and over a run both their product and the run's end state from zero can leave
+// float while the state itself does not (it may be 0 there, tiny, or cancelled by the run's first frames).  Without softplus the states in
+// front of the runs are therefore left by this kernel whatever their number, one run after the other: the factor meets the state with its
+// exponent apart, and a run whose result is not finite all the same is walked frame by frame from the state in front of it, as the uncut
+// scan does.  A lane owns one state.
+__device__ __forceinline__ float carried(float x, float e) {       // exp2(e) x
+    const float whole = floorf(e);
+    return x == 0.f ? 0.f : ldexpf(x * __builtin_amdgcn_exp2f(e - whole), (int)fminf(fmaxf(whole, -1000.f), 1000.f));
+}
+template <class S>
+__global__ __launch_bounds__(64) void scan_runs_careful_kernel(ScanArgs a, int NP, int back) {
+    const long long M = (long long)a.B * a.D * NP, m = (long long)blockIdx.x * 64 + threadIdx.x;
+    if (m >= M) return;
+    const long long bd = m / NP;
+    const int n = (int)(m % NP), d = (int)(bd % a.D), b = (int)(bd / a.D);
+    const bool real = n < a.N;
+    const float A2 = real ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : 0.f, bias = a.dbias ? a.dbias[d] : 0.f;
+    const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
+    auto walk = [&](int c, float x) {
+        const S *u = static_cast<const S*>(a.u) + b * a.ub + d, *e = static_cast<const S*>(a.delta) + b * a.eb + d;
+        const S *z = static_cast<const S*>(a.z) + b * a.zb + d, *g = static_cast<const S*>(a.dy) + b * a.gb + d;
+        const S *bm = static_cast<const S*>(a.b) + b * a.bb + n, *cm = static_cast<const S*>(a.c) + b * a.cb + n;
+        const int p0 = c * a.run, frames = min(min(p0 + a.run, a.T), len) - p0;
+        for (int i = 0; i < frames; ++i) {
+            const int p = back ? p0 + frames - 1 - i : p0 + i;
+            const long long f = a.reverse ? len - 1 - p : p;
+            const float D = step_of(a, (float)e[f * a.et] + bias), ex = __builtin_amdgcn_exp2f(D * A2);
+            if (back) {
+                float gi = (float)g[f * a.gt];
+                if (a.z) {
+                    const float zi = (float)z[f * a.zt];
+                    gi *= zi * fast_sigmoid(zi);
+                }
+                x = fmaf((float)cm[f * a.ct], gi, x) * ex;
+            } else x = fmaf(ex, x, D * (float)u[f * a.ut] * (float)bm[f * a.bt]);
+        }
+        return x;
+    };
+    const float* start = back ? a.dh_out : a.h0;
+    float x = start && real ? start[bd * a.N + n] : 0.f;
+    for (int k0 = 0; k0 < a.nrun; k0 += 8) {
+        float s[8], dt[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = back ? a.nrun - 1 - (k0 + i) : k0 + i;
+            const bool has = k0 + i < a.nrun - 1;                   // (nothing lies behind the last one: it left no end state)
+            s[i] = has ? a.runs[(long long)c * M + m] : 0.f;
+            dt[i] = has ? a.runs_dt[(long long)c * (M / NP) + bd] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = k0 + i, c = back ? a.nrun - 1 - k : k;
+            if (k < a.nrun) a.runs[(long long)c * M + m] = x;
+            if (k < a.nrun - 1) {
+                const float next = carried(x, dt[i] * A2) + s[i];
+                x = fabsf(next) <= 3.402823466e38f || x != x || !real ? next : walk(c, x);
+            }
+        }
     }
 }
 
@@ -986,11 +1047,12 @@ static int scan_check(const char* name, int T, int B, int D, int N, int dtype) {
     return PBSED_OK;
 }
 
-static int scan_fold(ScanArgs& a, const ScanPlan& p, int back, hipStream_t s) {
-    a.folded = p.nrun > SC_FOLD;
+template <class S> static int scan_fold(ScanArgs& a, const ScanPlan& p, int back, hipStream_t s) {
+    a.folded = p.nrun > SC_FOLD || !a.softplus;
     if (!a.folded) return PBSED_OK;
-    const long long blocks = ((long long)a.B * a.D * p.np + 63) / 64;
-    hipLaunchKernelGGL(scan_runs_kernel, dim3((unsigned)blocks), dim3(1024), 0, s, a, p.np, back);
+    const unsigned blocks = (unsigned)(((long long)a.B * a.D * p.np + 63) / 64);
+    if (a.softplus) hipLaunchKernelGGL(scan_runs_kernel, dim3(blocks), dim3(1024), 0, s, a, p.np, back);
+    else hipLaunchKernelGGL(scan_runs_careful_kernel<S>, dim3(blocks), dim3(64), 0, s, a, p.np, back);
     return check_launch("selective_scan runs");
 }
 template <class S, int LN, int NS>
@@ -998,7 +1060,7 @@ static int scan_fwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
         hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, true>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_fwd runs")) return rc;
-        if (const int rc = scan_fold(a, p, 0, s)) return rc;
+        if (const int rc = scan_fold<S>(a, p, 0, s)) return rc;
     }
     hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, false>), dim3(p.blocks, a.B, p.nrun), dim3(256), 0, s, a);
     return check_launch("selective_scan_fwd");
@@ -1008,7 +1070,7 @@ static int scan_bwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
         hipLaunchKernelGGL((scan_bwd_summary_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_bwd runs")) return rc;
-        if (const int rc = scan_fold(a, p, 1, s)) return rc;
+        if (const int rc = scan_fold<S>(a, p, 1, s)) return rc;
     }
     constexpr size_t lds = ScanBwdLds<LN, NS>::bytes;
     PBSED_DYN_LDS_ONCE((scan_bwd_kernel<S, LN, NS>), lds);

@@ -1,0 +1,94 @@
+"""The sequence operators of pb_sed_amd.ops at the edges of their ranges, against the float64 restatements of tests/sequence_ref.py: on the
+GPU and on the emulated device (whose eight CUs cut small cases into runs as well)."""
+import numpy as np
+import pytest
+import torch
+
+from tests import sequence_ref as ref
+from tests.sequence_ref import check
+from tests.test_sequence_ops import BF16, F16, F32, dev, emulated_library, lens, normal, rounded, scan_inputs, slot      # noqa: F401
+
+
+def up(v, dev):                                                       # noqa: F811
+    return {k: x.to(dev) for k, x in v.items()}
+
+
+def scan_forward(ops, v, n=None, **kw):
+    """(y, state behind the frames) of inputs ``v`` (frames from n[0] to n[1])."""
+    cut = {k: v[k][slice(*n)] if n else v[k] for k in ('u', 'delta', 'b', 'c')}
+    return ops.selective_scan_fwd(cut['u'], cut['delta'], v['a_log'], cut['b'], cut['c'], want_state=True, **kw)[:2]
+
+
+# ------------------------------------------------------------------------------------------------ scans that grow
+# softplus=False takes steps below zero, whose factors exp(D A) are above one: over a run of 48 frames (what T >= 128 frames of few clips
+# and channels are cut into) their product leaves float32 long before a result does.
+def growing(t, d, n, step=-3.):
+    g = torch.Generator().manual_seed(t + n)
+    v = dict(u=torch.zeros(t, 1, d), delta=torch.full((t, 1, d), step), b=normal(g, t, 1, n).float(), c=normal(g, t, 1, n).float(), a_log=torch.zeros(d, n),
+             dy=torch.zeros(t, 1, d))
+    return v
+
+
+@pytest.mark.parametrize('n', [4, 16, 20, 64])
+@pytest.mark.parametrize('reverse', [False, True])
+def test_growing_scans_cut_into_runs_stay_zero_until_they_are_driven(dev, n, reverse):      # noqa: F811
+    """390 silent frames whose factors multiply up to exp(1170), then ten of input: the state is 0 until then.  Backward: only the first
+    ten frames have a gradient, and the adjoint is 0 behind them."""
+    from pb_sed_amd import ops
+    t, d = 400, 5
+    v = growing(t, d, n)
+    last = slice(0, 10) if reverse else slice(390, 400)               # the last ten, the first ten frames in scan order
+    first = slice(390, 400) if reverse else slice(0, 10)
+    v['u'][last] = 1.
+    v['dy'][first] = 1.
+    x = up(v, dev)
+    want = ref.scan(*(v[k].double() for k in ('u', 'delta', 'a_log', 'b', 'c')), softplus=False, reverse=reverse, dy=v['dy'].double())
+    args = [x[k] for k in ('u', 'delta', 'a_log', 'b', 'c')]
+    y, state, saved = ops.selective_scan_fwd(*args, softplus=False, reverse=reverse, want_state=True, save=True)
+    k = 30 + 64                                                       # (as in test_sequence_ops: 30 per frame, a sum of D over a run)
+    check(y, want['y'], want['major']['y'], k, 'y')
+    check(state, want['state_out'], want['major']['state_out'], k, 'state_out')
+    silent = torch.ones(t, dtype=torch.bool)
+    silent[last] = False
+    assert (y.cpu()[silent] == 0).all()
+    da, dd, db = torch.zeros(d, n, device=dev), torch.zeros(d, device=dev), torch.zeros(d, device=dev)
+    got = ops.selective_scan_bwd(x['dy'], *args, saved, softplus=False, reverse=reverse, da_log=da, dd=dd, ddelta_bias=db, want_dstate=True)
+    k = 2 * k + 20 + 16 + t // 16
+    for key, value in (*zip(('du', 'ddelta', 'db', 'dc'), got), ('dstate', got[5]), ('da_log', da), ('dd', dd), ('ddelta_bias', db)):
+        check(value, want[key], want['major'][key], k, key)
+
+
+def test_growing_scans_do_not_depend_on_the_cut(dev):                 # noqa: F811
+    """The cut call, the same frames in uncut pieces and frame by frame: a state that is cancelled at the border of two runs, and one so
+    small that only the product of a run's factors with it is within float32."""
+    from pb_sed_amd import ops
+    t, d, n = 144, 3, 4
+    v = growing(t, d, n, step=0.)
+    v['a_log'].fill_(float(np.log(np.log(2.))))                       # factor 2^-D
+    v['b'].fill_(1.)
+    start = torch.zeros(1, d, n)
+    # channel 0: the state 1 meets -8 in frame 48 and would grow 8-fold in the 47 frames behind it, as would the input alone: 2^141
+    start[:, 0] = 1.
+    v['delta'][48:96, :, 0] = -3.
+    v['u'][48, :, 0] = 8 / 3
+    # channel 1: 2^-140 grows by 2^200 in frames 48 .. 95 and is held; channel 2: shrinks by 2^200, then grows by it
+    start[:, 1] = 2. ** -120
+    v['delta'][48:96, :, 1] = -200 / 48
+    start[:, 2] = 2. ** 100
+    v['delta'][:48, :, 2] = 200 / 48
+    v['delta'][48:96, :, 2] = -200 / 48
+    x, h0 = up(v, dev), start.to(dev)
+    want = ref.scan(*(v[k].double() for k in ('u', 'delta', 'a_log', 'b', 'c')), softplus=False, state=start.double())
+    y, state = scan_forward(ops, x, softplus=False, state=h0)
+    check(y, want['y'], want['major']['y'], 94, 'y')
+    check(state, want['state_out'], want['major']['state_out'], 94, 'state_out')
+    pieces, h = [], h0
+    for a in range(0, t, 36):                                         # 36 frames are not cut
+        p, h = scan_forward(ops, x, (a, a + 36), softplus=False, state=h)
+        pieces.append(p)
+    check(torch.cat(pieces), want['y'], want['major']['y'], 94, 'y in pieces')
+    h = h0.clone()
+    for f in range(t):
+        one = ops.selective_scan_step(x['u'][f], x['delta'][f], x['a_log'], x['b'][f], x['c'][f], h, softplus=False)
+        check(one, want['y'][f], want['major']['y'][f], 94, f'frame {f}')
+    check(h, want['state_out'], want['major']['state_out'], 94, 'state, frame by frame')
