@@ -8,6 +8,9 @@
 //     ddelta = dD sigmoid(raw),   da_log = A sum_{t,b} r D q,   dskip = sum g u,   dz = dy (C.h + skip u) silu'(z)
 // Frames behind a clip's end are not read, their outputs are 0, and the state stands still.
 //
+// An infinity stays what the formula makes of it: states behind N and channels behind D take part in the lanes' work as zeros whose inputs are
+// zeros too (a row of LDS that holds nothing else), and never as zeros beside an infinite D, u, g, B or C - their product would be NaN.
+//
 // Layout: LN lanes share a channel, NS states each (N <= 8: 4 x 2, <= 16: 8 x 2, <= 32: 16 x 2, <= 64: 16 x 4), so a wave holds
 // 64 / LN channels and its states never leave registers; y is a sum of NS terms per lane and log2(LN) DPP adds.  A block of four waves
 // stages a tile of frames: softplus, the products with u and the gate are computed once per element, coalesced along the channels, and
@@ -131,7 +134,14 @@ __device__ __forceinline__ float rate_of(float a_log) {
     const float v = expf(a_log);
     return v > 1e37f ? 1e37f : v;
 }
+// -rate log2(e) of a lane's states; -1 for states that do not exist (a run's infinite sum of D takes their zero to zero, not to NaN)
+template <int NS> __device__ __forceinline__ void rates2(const ScanArgs& a, int d, int n0, float (&A2)[NS]) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j) A2[j] = d < a.D && n0 + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n0 + j]) : -1.f;
+}
 __device__ __forceinline__ float step_of(const ScanArgs& a, float raw) { return a.softplus ? softplus(raw) : raw; }
+// v, or 0 (mask 0: what meets a weight that is not there)
+__device__ __forceinline__ float masked(float v, unsigned mask) { return __uint_as_float(__float_as_uint(v) & mask); }
 // D of F frames of a channel, 0 for those that do not exist (frames F sq + i >= left of a tile); the uniform choices stand outside, so that
 // the F chains interleave
 template <int F> __device__ __forceinline__ void steps_of(const ScanArgs& a, const float (&raw)[F], float bias, int first, int left, float (&D)[F]) {
@@ -175,7 +185,7 @@ __global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int
     const bool on = m < M;
     const long long bd = on ? m / NP : 0;
     const int n = (int)(m % NP), d = (int)(bd % a.D);
-    const float A2 = on && n < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : 0.f;
+    const float A2 = on && n < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : -1.f;
     const float* start = back ? a.dh_out : a.h0;
     const float x0 = start && on && n < a.N ? start[bd * a.N + n] : 0.f;
     float s[16], dt[16], S = 0.f, P = 0.f;
@@ -220,7 +230,7 @@ __global__ __launch_bounds__(64) void scan_runs_careful_kernel(ScanArgs a, int N
     const long long bd = m / NP;
     const int n = (int)(m % NP), d = (int)(bd % a.D), b = (int)(bd / a.D);
     const bool real = n < a.N;
-    const float A2 = real ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : 0.f, bias = a.dbias ? a.dbias[d] : 0.f;
+    const float A2 = real ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + n]) : -1.f, bias = a.dbias ? a.dbias[d] : 0.f;
     const int len = a.seq_len ? min(max(a.seq_len[b], 0), a.T) : a.T;
     auto walk = [&](int c, float x) {
         const S *u = static_cast<const S*>(a.u) + b * a.ub + d, *e = static_cast<const S*>(a.delta) + b * a.eb + d;
@@ -356,6 +366,8 @@ template <class S, int CB> __device__ __forceinline__ ScanBlock scan_block() {
     return ScanBlock{(int)(w % gridDim.x), (int)(w / gridDim.x % gridDim.y), (int)(w / gridDim.x / gridDim.y)};
 }
 
+// lanes of a kernel may have no state or channel
+template <int LN, bool MIX> constexpr bool spare_lanes = MIX || LN < 16;
 // LDS operands of four frames of the compute phase, read one group ahead of their use
 template <int NS, bool C> struct ScanGroup {
     float4 D, U;
@@ -371,15 +383,20 @@ template <int NS, bool C> struct ScanGroup {
     }
 };
 
-// grid (channel blocks, B, runs).  SUMMARY: leave this run's end state from zero and sum of D; otherwise the outputs.
-template <class S, int LN, int NS, bool SUMMARY>
+// grid (channel blocks, B, runs).  SUMMARY: leave this run's end state from zero and sum of D; otherwise the outputs.  Lanes without a
+// state read zeros for D and U.  MIX: N is no multiple of NS, so that a lane holds states that exist beside some that do not; those are
+// selected to zero.  (For LN = 16, whose registers are all taken, MIX also stands for the lanes without a state or channel, and the other
+// form has none: 500 frames x 16 x 256 float, N = 32: 122 us with the zeros' pointers, 118 without, N = 64: 240 and 230.)
+template <class S, int LN, int NS, bool SUMMARY, bool MIX>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
     constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4, W = lane_frames<LN>;
     using Rows = LaneRows<S, 4>;
     using BC = StateRows<S, TT, NP>;
     __shared__ __attribute__((aligned(16))) float sD[2][CB * LD], sU[2][CB * LD], sB[2][TT * NP], sC[2][SUMMARY ? 4 : TT * NP];
+    __shared__ __attribute__((aligned(16))) float nothing[TT];    // zeros: the row of lanes without a state
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     const int ch = wave * (64 / LN) + lane / LN;                 // the lane's channel of the block
+    if (tid < TT) nothing[tid] = 0.f;
     const ScanBlock blk = scan_block<S, CB>();
     const int b = blk.b, c = blk.c, d0 = blk.x * CB, d = d0 + ch;
     const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;       // staging: channel, group of four frames
@@ -399,10 +416,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
     const Rows oz(a.zt, TT, sq, sch, a.reverse, chan & gated), oy(yt, TT, sq, sch, a.reverse, chan);
     const BC ob(a.bt, a.N, a.reverse), oc(a.ct, a.N, a.reverse);
     const float bias = chan && a.dbias ? a.dbias[sd] : 0.f, skip = chan && a.skip ? a.skip[sd] : 0.f;
+    const unsigned skip_mask = a.skip ? ~0u : 0u;
 
     float A2[NS], h[NS] = {}, dsum = 0.f;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) A2[j] = d < a.D && nq * NS + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
+    rates2<NS>(a, d, nq * NS, A2);
     if (!SUMMARY && d < a.D) {
         if (a.h0) load_states<NS>(a.h0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, h);
         if (a.nrun > 1) fold_runs<LN, NS>(a, c, 0, c, 1, b, d, nq, A2, h);
@@ -453,8 +470,9 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
         if (!SUMMARY) oc.put(sC[buf], rc);
         __syncthreads();
         if (t0 + TT < stop) fetch(len - t0 - TT);
-        float* rowD = &sD[buf][ch * LD];
-        const float* rowU = &sU[buf][ch * LD];
+        float* out = &sD[buf][ch * LD];                            // where the sums over the channel's states go
+        const bool with = !spare_lanes<LN, MIX> || nq * NS < a.N;
+        const float *rowD = with ? out : nothing, *rowU = with ? &sU[buf][ch * LD] : nothing;
         ScanGroup<NS, !SUMMARY> g;
         g.template load<NP>(rowD, rowU, sB[buf], sC[buf], 0, nq);
 #pragma unroll
@@ -477,6 +495,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
                     h[j] = fmaf(ex[i][j], h[j], x[i][j]);
+                    if (MIX && j) h[j] = nq * NS + j < a.N ? h[j] : 0.f;
                     if constexpr (!SUMMARY) y4[i] = j ? fmaf(g.Cv[i].v[j], h[j], y4[i]) : g.Cv[i].v[j] * h[j];
                 }
                 if (SUMMARY) dsum += at(g.D, i);
@@ -487,7 +506,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 #pragma unroll
                 for (int i = 0; i < W; ++i) yw[i] = y4[i];
                 arrived(yw);
-                if (nq % 4 == 0) store_pack<float, W>(rowD + 4 * q + nq / 4 * W, yw);      // the channel's lanes have read D there
+                if (nq % 4 == 0) store_pack<float, W>(out + 4 * q + nq / 4 * W, yw);       // the channel's lanes have read D there
             }
             if (q + 1 < TT / 4) g = next;
         }
@@ -496,7 +515,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
         float o[4];
         load_pack<float, 4>(&sD[buf][sch * LD + sq * 4], o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(uc[i], skip, o[i]) * gate[i];
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(masked(uc[i], skip_mask), skip, o[i]) * gate[i];
         oy.template store<false>(rows_at(y), sq, len - t0, o);
         y += adv * yt;
     }
@@ -516,14 +535,16 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // adjoint from behind a run: what the run's own dy leave on the state in front of it (runs), and its sum of D
-template <class S, int LN, int NS>
+template <class S, int LN, int NS, bool MIX>
 __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
     constexpr int NP = NS * LN, CB = 256 / LN, TT = 1024 / CB, LD = TT + 4;
     using Rows = LaneRows<S, 4>;
     using BC = StateRows<S, TT, NP>;
     __shared__ __attribute__((aligned(16))) float sD[2][CB * LD], sG[2][CB * LD], sC[2][TT * NP];
+    __shared__ __attribute__((aligned(16))) float nothing[TT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     const int ch = wave * (64 / LN) + lane / LN;
+    if (tid < TT) nothing[tid] = 0.f;
     const ScanBlock blk = scan_block<S, CB>();
     const int b = blk.b, c = blk.c + 1, d0 = blk.x * CB, d = d0 + ch;         // run 0 has nothing in front of it
     const int sch = tid % CB, sq = tid / CB, sd = d0 + sch;
@@ -540,8 +561,7 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
     const BC oc(a.ct, a.N, a.reverse);
     const float bias = chan && a.dbias ? a.dbias[sd] : 0.f;
     float A2[NS], r[NS] = {}, dsum = 0.f;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) A2[j] = d < a.D && nq * NS + j < a.N ? -LOG2E * rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
+    rates2<NS>(a, d, nq * NS, A2);
     arrived(A2);
     Raw<S> re[4], rz[4], rg[4], rc[BC::NB];
     auto request = [&](auto full, int left) __attribute__((always_inline)) {
@@ -570,7 +590,8 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
         oc.put(sC[buf], rc);
         __syncthreads();
         if (t0 - TT >= p0) fetch(len - t0 + TT);
-        const float *rowD = &sD[buf][ch * LD], *rowG = &sG[buf][ch * LD];
+        const bool with = !spare_lanes<LN, MIX> || nq * NS < a.N;
+        const float *rowD = with ? &sD[buf][ch * LD] : nothing, *rowG = with ? &sG[buf][ch * LD] : nothing;
         ScanGroup<NS, false> gr;                                 // (D, g, C in the places of D, U, B)
         gr.template load<NP>(rowD, rowG, sC[buf], nullptr, TT / 4 - 1, nq);
 #pragma unroll
@@ -586,7 +607,10 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
 #pragma unroll
-                for (int j = 0; j < NS; ++j) r[j] = fmaf(gr.B[i].v[j], at(gr.U, i), r[j]) * ex[i][j];
+                for (int j = 0; j < NS; ++j) {
+                    r[j] = fmaf(gr.B[i].v[j], at(gr.U, i), r[j]) * ex[i][j];
+                    if (MIX && j) r[j] = nq * NS + j < a.N ? r[j] : 0.f;
+                }
                 dsum += at(gr.D, i);
             }
             if (q) gr = next;
@@ -634,13 +658,14 @@ __device__ __forceinline__ void channel_sums(const float (&vB)[NS], const float 
 // channels x 16 states, float, under sustained load): forward 51 us, backward 118 us with its sums (whole sums in every lane 129).
 template <int LN, int NS> struct ScanBwdLds {
     static constexpr int NP = NS * LN, CB = 256 / LN, TT = SC_SAVE, LD = TT + 4, F = CB * TT / 256;
-    static constexpr int rows = CB * LD, bc = TT * NP, part = 4 * TT * 2 * NP, keep = 5 * 256 * F;
+    static constexpr int rows = (CB + 1) * LD, bc = TT * NP, part = 4 * TT * 2 * NP, keep = 5 * 256 * F;
     static constexpr int parts = NP <= 32 ? 2 : 1;               // buffers of the sums: with one, a tile ends with a second barrier
-    static constexpr size_t bytes = (size_t)(3 * rows + 4 * bc + parts * part + keep) * sizeof(float);
+    // sD, sU, sG (with a last row of zeros); B and C of two tiles, and zeros in their place for lanes without a channel; sums; what a thread keeps
+    static constexpr size_t bytes = (size_t)(3 * rows + 5 * bc + parts * part + keep) * sizeof(float);
 };
 // (three blocks per CU: 168 registers, which four lanes per channel and four states per lane overrun - N = 8: forward and backward of
 // 500 x 32 x 512 float 204 us with three, 170 with two)
-template <class S, int LN, int NS>
+template <class S, int LN, int NS, bool MIX>
 __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kernel(ScanArgs a) {
     using L = ScanBwdLds<LN, NS>;
     constexpr int NP = L::NP, CB = L::CB, TT = L::TT, LD = L::LD, F = L::F, W = lane_frames<LN>;                  // F frames of a channel per thread and tile
@@ -649,7 +674,7 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
     using BC = StateRows<S, TT, NP>;
     static_assert(F >= 1 && NP2 >= 1 && L::rows >= 256, "a tile has work for every thread");
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *lds_bc = sG + L::rows, *lds_part = lds_bc + 4 * L::bc;     // [2][B | C], [parts][4][TT][2 NP]
+    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *lds_bc = sG + L::rows, *nothing = lds_bc + 4 * L::bc, *lds_part = nothing + L::bc;     // [2][B | C], [parts][4][TT][2 NP]
     Pack<float, F>* keep = reinterpret_cast<Pack<float, F>*>(lds_part + L::parts * L::part) + threadIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     constexpr int WC = 64 / LN;                                  // channels of a wave: it stages them for itself
@@ -684,13 +709,19 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
         op[k] = ((unsigned)(a.reverse ? TT - 1 - m : m) * (unsigned)(a.B * 2 * NP) + (unsigned)(i % (2 * NP))) * 4u;
     }
     const float bias = chan && a.dbias ? a.dbias[sd] : 0.f, skip = chan && a.skip ? a.skip[sd] : 0.f;
+    const unsigned skip_mask = a.skip ? ~0u : 0u;
     float dskip = 0.f, dbias = 0.f;
     float A2[NS], A[NS], r[NS] = {}, da[NS] = {};
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
         A[j] = d < a.D && nq * NS + j < a.N ? -rate_of(a.a_log[(long long)d * a.N + nq * NS + j]) : 0.f;
-        A2[j] = A[j] * LOG2E;
+        A2[j] = d < a.D && nq * NS + j < a.N ? A[j] * LOG2E : -1.f;
     }
+    const bool with = !spare_lanes<LN, MIX> || (d < a.D && nq * NS < a.N);    // the lane has a channel and a state
+    const float *rowD = sD + (with ? ch : CB) * LD, *rowU = rowD + L::rows, *rowG = rowU + L::rows, *bc0 = with ? lds_bc : nothing;
+    const int bc_buf = with ? 2 * L::bc : 0, bc_c = with ? L::bc : 0;         // from B of the tile before to this one's, from B to C
+    for (int i = tid; i < L::bc; i += 256) nothing[i] = 0.f;
+    if (tid < LD) sD[CB * LD + tid] = sU[CB * LD + tid] = sG[CB * LD + tid] = 0.f;
     if (d < a.D) {
         if (a.dh_out) load_states<NS>(a.dh_out + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
         if (a.nrun > 1) fold_runs<LN, NS>(a, c, a.nrun - 1, c, -1, b, d, nq, A2, r);
@@ -771,26 +802,31 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
         for (int j = 0; j < NS; ++j) h[j] = rh[j];
         wave_handover();
         if (t0 - TT >= p0) fetch(len - t0 + TT);
-        float *rowD = sD + ch * LD, *rowU = sU + ch * LD, *rowG = sG + ch * LD;
+        const float *rowB = bc0 + buf * bc_buf, *rowC = rowB + bc_c;
+        float *outD = sD + ch * LD, *outU = outD + L::rows, *outG = outU + L::rows;       // where the sums over the channel's states go
         float ex[TT][NS], hs[TT][NS], h0[NS];                    // hs[t]: the state behind frame t
 #pragma unroll
         for (int j = 0; j < NS; ++j) h0[j] = h[j];
         ScanGroup<NS, false> gr;
-        gr.template load<NP>(rowD, rowU, sB, nullptr, 0, nq);
+        gr.template load<NP>(rowD, rowU, rowB, nullptr, 0, nq);
 #pragma unroll
         for (int k = 0; k < TT / 4; ++k) {
             ScanGroup<NS, false> next;
-            if (k + 1 < TT / 4) next.template load<NP>(rowD, rowU, sB, nullptr, k + 1, nq);
+            if (k + 1 < TT / 4) next.template load<NP>(rowD, rowU, rowB, nullptr, k + 1, nq);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < NS; ++j) ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
+                for (int j = 0; j < NS; ++j) {
+                    ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
+                    if (MIX && j) ex[4 * k + i][j] = nq * NS + j < a.N ? ex[4 * k + i][j] : 0.f;
+                }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
                     h[j] = fmaf(ex[4 * k + i][j], h[j], at(gr.U, i) * gr.B[i].v[j]);
+                    if (MIX && j) h[j] = nq * NS + j < a.N ? h[j] : 0.f;
                     hs[4 * k + i][j] = h[j];
                 }
             if (k + 1 < TT / 4) gr = next;
@@ -799,7 +835,7 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
 #pragma unroll
         for (int k = TT / 4 - 1; k >= 0; --k) {
             ScanGroup<NS, true> gb;
-            gb.template load<NP>(rowD, rowU, sB, sC, k, nq);
+            gb.template load<NP>(rowD, rowU, rowB, rowC, k, nq);
             const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
             __builtin_amdgcn_sched_barrier(0);
             float o12[12];                                       // (k, b, y) of four frames
@@ -810,7 +846,9 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
                 float vB[NS], vC[NS], v[NS / 2];
 #pragma unroll
                 for (int j = 0; j < NS; ++j) {
-                    const float rj = fmaf(gb.Cv[i].v[j], gi, r[j]), hj = hs[s][j];
+                    float rj = fmaf(gb.Cv[i].v[j], gi, r[j]);
+                    if (MIX && j) rj = nq * NS + j < a.N ? rj : 0.f;
+                    const float hj = hs[s][j];
                     r[j] = rj * ex[s][j];
                     const float rq = r[j] * (s ? hs[s ? s - 1 : 0][j] : h0[j]);
                     o12[2 + 3 * i] = j ? fmaf(gb.Cv[i].v[j], hj, o12[2 + 3 * i]) : gb.Cv[i].v[j] * hj;
@@ -838,9 +876,9 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
             arrived(yo);
             if (nq % 4 == 0) {                                   // the channel's lanes have read these four frames
                 const int at_ = 4 * k + nq / 4 * W;
-                store_pack<float, W>(rowD + at_, ko);
-                store_pack<float, W>(rowU + at_, bo);
-                store_pack<float, W>(rowG + at_, yo);
+                store_pack<float, W>(outD + at_, ko);
+                store_pack<float, W>(outU + at_, bo);
+                store_pack<float, W>(outG + at_, yo);
             }
         }
 #pragma unroll
@@ -857,8 +895,8 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
 #pragma unroll
         for (int i = 0; i < F; ++i) {
             xe[i] = fmaf(ku.v[i], bb.v[i], kk.v[i]) * kS.v[i];
-            xu[i] = fmaf(kG.v[i], skip, kD.v[i] * bb.v[i]);
-            xz[i] = kZ.v[i] * fmaf(skip, ku.v[i], yy.v[i]);
+            xu[i] = fmaf(masked(kG.v[i], skip_mask), skip, kD.v[i] * bb.v[i]);
+            xz[i] = kZ.v[i] * fmaf(skip, masked(ku.v[i], skip_mask), yy.v[i]);
             tile_bias += sq * F + i < len - t0 ? xe[i] : 0.f;
         }
         dbias += tile_bias;
@@ -981,7 +1019,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], du * (float)f.B.v[j]);
-            y = fmaf((float)f.C.v[j], h[j], y);
+            y = (WHOLE ? has : n0 + j < a.N) ? fmaf((float)f.C.v[j], h[j], y) : y;
         }
         y = lanes_sum<LN>(y);
         if (on) {
@@ -990,7 +1028,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
                 if (has) store_loose<float, NS>(out + n0, h);
             } else store_states<NS>(out, n0, a.N, h);
             if (n0 == 0) {
-                y = fmaf(skip, u, y);
+                if (a.skip) y = fmaf(skip, u, y);
                 static_cast<S*>(a.y)[(long long)b * a.D + d] = (S)(a.z ? y * (z * fast_sigmoid(z)) : y);
             }
         }
@@ -1055,26 +1093,26 @@ template <class S> static int scan_fold(ScanArgs& a, const ScanPlan& p, int back
     else hipLaunchKernelGGL(scan_runs_careful_kernel<S>, dim3(blocks), dim3(64), 0, s, a, p.np, back);
     return check_launch("selective_scan runs");
 }
-template <class S, int LN, int NS>
+template <class S, int LN, int NS, bool MIX>
 static int scan_fwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
-        hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, true>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, true, MIX>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_fwd runs")) return rc;
         if (const int rc = scan_fold<S>(a, p, 0, s)) return rc;
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, false>), dim3(p.blocks, a.B, p.nrun), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((scan_fwd_kernel<S, LN, NS, false, MIX>), dim3(p.blocks, a.B, p.nrun), dim3(256), 0, s, a);
     return check_launch("selective_scan_fwd");
 }
-template <class S, int LN, int NS>
+template <class S, int LN, int NS, bool MIX>
 static int scan_bwd_launch(ScanArgs& a, const ScanPlan& p, hipStream_t s) {
     if (p.nrun > 1) {
-        hipLaunchKernelGGL((scan_bwd_summary_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((scan_bwd_summary_kernel<S, LN, NS, MIX>), dim3(p.blocks, a.B, p.nrun - 1), dim3(256), 0, s, a);
         if (const int rc = check_launch("selective_scan_bwd runs")) return rc;
         if (const int rc = scan_fold<S>(a, p, 1, s)) return rc;
     }
     constexpr size_t lds = ScanBwdLds<LN, NS>::bytes;
-    PBSED_DYN_LDS_ONCE((scan_bwd_kernel<S, LN, NS>), lds);
-    hipLaunchKernelGGL((scan_bwd_kernel<S, LN, NS>), dim3(p.blocks, a.B, p.nrun), dim3(256), lds, s, a);
+    PBSED_DYN_LDS_ONCE((scan_bwd_kernel<S, LN, NS, MIX>), lds);
+    hipLaunchKernelGGL((scan_bwd_kernel<S, LN, NS, MIX>), dim3(p.blocks, a.B, p.nrun), dim3(256), lds, s, a);
     return check_launch("selective_scan_bwd");
 }
 template <class S, int LN>
@@ -1089,11 +1127,13 @@ static int scan_step_launch(ScanArgs& a, hipStream_t s) {
     return check_launch("selective_scan_step");
 }
 
+#define PBSED_SCAN_MIX(launch, LN, NS) \
+    (N % NS || (LN == 16 && (N != LN * NS || D % (256 / LN))) ? launch<S, LN, NS, true>(a, p, s) : launch<S, LN, NS, false>(a, p, s))
 #define PBSED_SCAN(launch)                                                    \
-    PBSED_ELEM(dtype, rc = p.ln == 4 ? launch<S, 4, 2>(a, p, s)               \
-                           : p.ln == 8 ? launch<S, 8, 2>(a, p, s)             \
-                           : p.ns == 2 ? launch<S, 16, 2>(a, p, s)            \
-                                       : launch<S, 16, 4>(a, p, s))
+    PBSED_ELEM(dtype, rc = p.ln == 4 ? PBSED_SCAN_MIX(launch, 4, 2)           \
+                           : p.ln == 8 ? PBSED_SCAN_MIX(launch, 8, 2)         \
+                           : p.ns == 2 ? PBSED_SCAN_MIX(launch, 16, 2)        \
+                                       : PBSED_SCAN_MIX(launch, 16, 4))
 
 }  // namespace pbsed
 

@@ -92,3 +92,71 @@ def test_growing_scans_do_not_depend_on_the_cut(dev):                 # noqa: F8
         one = ops.selective_scan_step(x['u'][f], x['delta'][f], x['a_log'], x['b'][f], x['c'][f], h, softplus=False)
         check(one, want['y'][f], want['major']['y'][f], 94, f'frame {f}')
     check(h, want['state_out'], want['major']['state_out'], 94, 'state, frame by frame')
+
+
+# ------------------------------------------------------------------------------------------------ infinities beside padding
+# States are padded to 8, 16, 32 or 64 and channels to a block; an infinity that the formula keeps must not meet their zeros.
+def same(got, want, what):
+    """NaN, infinities and their signs as in the formula.  The rest: at most 237 roundings (2 (30 + 64) of a state and an adjoint, 49 of the
+    sums) against majorants that exceed these positive sums at most 20-fold (1 + the sum of D rate <= 19): 3e-4."""
+    got = got.detach().cpu().double()
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(want)), (what, kind.__name__, kind(got).nonzero()[:5].tolist(), kind(want).nonzero()[:5].tolist())
+    fin = torch.isfinite(want)
+    err = (got[fin] - want[fin]).abs()
+    assert (err <= 3e-4 * want[fin].abs().clamp(min=1e-30)).all(), (what, float((err / want[fin].abs().clamp(min=1e-30)).max()))
+
+
+@pytest.mark.parametrize('n', [1, 3, 5, 8, 9, 12, 16, 19, 20, 33, 50, 62])
+@pytest.mark.parametrize('t', [32, 160])                              # 160: cut into runs
+@pytest.mark.parametrize('where', ['u', 'delta', 'b', 'c', 'dy'])
+def test_infinities_do_not_meet_the_padding(dev, n, t, where):        # noqa: F811
+    from pb_sed_amd import ops
+    d = 33 if t == 32 else 5
+    g = torch.Generator().manual_seed(n)
+    v = dict(u=(t, 1, d), delta=(t, 1, d), b=(t, 1, n), c=(t, 1, n), dy=(t, 1, d), d=(d,), delta_bias=(d,))
+    v = {k: .5 + torch.rand(*s, generator=g) for k, s in v.items()}
+    v['delta_bias'] -= 1.5
+    v['a_log'] = torch.full((d, n), -2.5)                             # D rate <= 0.13
+    v[where][{'c': 12, 'dy': 12}.get(where, 7), 0, 0 if where in 'bc' else 2] = float('inf')
+    want = ref.scan(*(v[k].double() for k in ('u', 'delta', 'a_log', 'b', 'c')), dy=v['dy'].double(), d=v['d'].double(), delta_bias=v['delta_bias'].double())
+    x = up(v, dev)
+    args, kw = [x[k] for k in ('u', 'delta', 'a_log', 'b', 'c')], dict(d=x['d'], delta_bias=x['delta_bias'])
+    y, state, saved = ops.selective_scan_fwd(*args, want_state=True, save=True, **kw)
+    same(y, want['y'], 'y')
+    same(state, want['state_out'], 'state_out')
+    da, dd, db = torch.zeros(d, n, device=dev), torch.zeros(d, device=dev), torch.zeros(d, device=dev)
+    got = ops.selective_scan_bwd(x['dy'], *args, saved, da_log=da, dd=dd, ddelta_bias=db, want_dstate=True, **kw)
+    for key, value in (*zip(('du', 'db', 'dc'), (got[0], *got[2:4])), ('dstate', got[5]), ('dd', dd)):
+        same(value, want[key], key)
+    for key, value in (('ddelta', got[1]), ('da_log', da), ('ddelta_bias', db)):         # (differences)
+        assert torch.equal(torch.isfinite(value.cpu()), torch.isfinite(want[key])), key
+    h = torch.zeros(1, d, n, device=dev)
+    for f in range(20 if where in ('u', 'delta', 'b', 'c') else 0):
+        one = ops.selective_scan_step(x['u'][f], x['delta'][f], x['a_log'], x['b'][f], x['c'][f], h, **kw)
+        same(one, want['y'][f], f'frame {f}')
+
+
+def test_infinities_without_the_skip_weight(dev):                     # noqa: F811
+    """d=None: there is no term for it, and none whose 0 an infinite input or gradient could meet."""
+    from pb_sed_amd import ops
+    g = torch.Generator().manual_seed(1)
+    t, d, n = 20, 5, 8
+    u, delta, b, c, z, dy = (.5 + torch.rand(t, 1, k, generator=g) for k in (d, d, n, n, d, d))
+    u[7, 0, 2], dy[12, 0, 3] = float('inf'), float('inf')
+    a_log = torch.full((d, n), -2.5)
+    u, delta, a_log, b, c, z, dy = (v.to(dev) for v in (u, delta, a_log, b, c, z, dy))
+    y, _, saved = ops.selective_scan_fwd(u, delta, a_log, b, c, z=z, save=True)
+    du, _, _, _, dz, _ = ops.selective_scan_bwd(dy, u, delta, a_log, b, c, saved, z=z)
+    inf = torch.zeros(t, 1, d, dtype=torch.bool)
+    inf[7:, 0, 2] = True                                              # the state is infinite from there on
+    assert torch.equal(torch.isposinf(y.cpu()), inf) and torch.isfinite(y.cpu()[~inf]).all()
+    inf[12, 0, 3] = True
+    assert torch.equal(torch.isposinf(dz.cpu()), inf) and torch.isfinite(dz.cpu()[~inf]).all()
+    inf.zero_()
+    inf[:13, 0, 3] = True                                             # the adjoint is, up to there
+    assert torch.equal(torch.isposinf(du.cpu()), inf) and torch.isfinite(du.cpu()[~inf]).all()
+    h = torch.zeros(1, d, n, device=dev)
+    for f in range(10):
+        one = ops.selective_scan_step(u[f], delta[f], a_log, b[f], c[f], h, z=z[f])
+        assert torch.equal(torch.isposinf(one.cpu()), torch.isposinf(y[f].cpu())) and not torch.isnan(one).any(), f
