@@ -437,7 +437,9 @@ int pbsed_event_frames(const float* scores, const float* thr, const int* len, in
  * (`dtype`), unit stride over channels, strides over frames and clips in elements; parameters, states and parameter gradients are
  * float.  seq_len [B] or NULL (= T): frames behind it are not read and their outputs are 0; `reverse` != 0 scans a clip's valid
  * frames from the last to the first.  Parameter gradients are ADDED to their buffers (any may be NULL), in a fixed order: results
- * are reproducible.  Workspaces are the caller's, used only by the launches of the call.  Limits (an error code and a message beyond
+ * are reproducible.  Workspaces are the caller's, used only by the launches of the call.  What a call writes must not share memory with
+ * what it reads or with another of its outputs: refused, but for dx / dz beside the activations (they may be channels of one wider
+ * buffer, whose disjointness is the caller's to check) and for what is said to be allowed below.  Limits (an error code and a message beyond
  * them): T <= 2^28, B <= 65535; convolution D <= 2^22; scan N <= 64, D (N + 2) < 2^26, frame strides < 2^23; layer norm rows < 2^30 of at
  * most 2^24 elements; fewer than 2^32 threads in a launch's dimension. */
 #define PBSED_F32 0

@@ -361,6 +361,11 @@ extern "C" int pbsed_causal_conv_fwd(const void* x, const float* w, const float*
                                      int silu, int reverse, int dtype, void* stream) {
     if (const int rc = cconv_check("causal_conv_fwd", T, B, D, K, dtype)) return rc;
     if (!x || !w || !y) { set_error("causal_conv_fwd: null pointer"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);
+    const long long whole = (long long)T * B * D * es, states = (long long)B * (K - 1) * D * es;
+    if (const int rc = ranges_apart("causal_conv_fwd", {{"y", y, whole}, {"state_out", state_out, states}},
+                                    {range3("x", x, T, x_stride_t, B, x_stride_b, D, es), {"weight", w, 4ll * D * K}, {"bias", bias, 4ll * D},
+                                     {"seq_len", seq_len, 4ll * B}, {"state", state, states}})) return rc;
     CConvArgs a{};
     a.x = x; a.w = w; a.bias = bias; a.seq_len = seq_len; a.state = state; a.y = y; a.state_out = state_out;
     a.T = T; a.B = B; a.D = D; a.xt = x_stride_t; a.xb = x_stride_b; a.yt = (long long)B * D; a.yb = D;
@@ -385,6 +390,16 @@ extern "C" int pbsed_causal_conv_bwd(const void* dy, const void* x, const float*
         set_error("causal_conv_bwd: the weight gradients need a workspace of %lld floats, got %lld", pbsed_causal_conv_workspace(T, B, D, K), ws_floats);
         return PBSED_E_ARG;
     }
+    const size_t es = elem_size(dtype);
+    const long long states = (long long)B * (K - 1) * D * es;
+    if (const int rc = ranges_apart("causal_conv_bwd", {{"dweight", dw, 4ll * D * K}, {"dbias", db, 4ll * D}, {"dstate", dstate, states},
+                                                        {"workspace", sums ? ws : nullptr, 4 * ws_floats}},
+                                    {range3("dx", dx, T, dx_stride_t, B, dx_stride_b, D, es), range3("x", x, T, x_stride_t, B, x_stride_b, D, es),
+                                     range3("dy", dy, T, dy_stride_t, B, dy_stride_b, D, es), {"weight", w, 4ll * D * K}, {"bias", bias, 4ll * D},
+                                     {"seq_len", seq_len, 4ll * B}, {"state", state, states}, {"dstate_out", dstate_out, states}})) return rc;
+    if (const int rc = ranges_apart("causal_conv_bwd", {range3("dx", dx, T, dx_stride_t, B, dx_stride_b, D, es)},
+                                    {{"weight", w, 4ll * D * K}, {"bias", bias, 4ll * D}, {"seq_len", seq_len, 4ll * B}, {"state", state, states},
+                                     {"dstate_out", dstate_out, states}})) return rc;
     CConvArgs a{};
     a.x = x; a.dy = dy; a.w = w; a.bias = bias; a.seq_len = seq_len; a.state = state; a.dstate_out = dstate_out; a.y = dx; a.state_out = dstate;
     a.ws = sums ? ws : nullptr;
@@ -404,6 +419,11 @@ extern "C" int pbsed_causal_conv_step(const void* x, const float* w, const float
                                       int D, int K, long long x_stride_b, int silu, int dtype, void* stream) {
     if (const int rc = cconv_check("causal_conv_step", 1, B, D, K, dtype)) return rc;
     if (!x || !w || !state || !state_out || !y) { set_error("causal_conv_step: null pointer"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);
+    const long long states = (long long)B * (K - 1) * D * es;
+    if (const int rc = ranges_apart("causal_conv_step", {{"y", y, (long long)B * D * (long long)es}, {"state_out", state_out, states}},
+                                    {range3("x", x, 1, 0, B, x_stride_b, D, es), {"weight", w, 4ll * D * K}, {"bias", bias, 4ll * D},
+                                     {"state", state == state_out ? nullptr : state, states}})) return rc;
     const long long grid = ((long long)B * D + 255) / 256;
     if (grid > CC_BLOCKS) { set_error("causal_conv_step: B = %d, D = %d need more than %lld blocks", B, D, CC_BLOCKS); return PBSED_E_UNSUPPORTED; }
     PBSED_ELEM(dtype, hipLaunchKernelGGL(causal_conv_step_kernel<S>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, static_cast<const S*>(x),

@@ -136,6 +136,8 @@ extern "C" int pbsed_dropout(const void* x, const void* residual, void* y, long 
         return PBSED_E_ARG;
     }
     if (!x || !y || !rng) { set_error("dropout: null pointer"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);                     // (x and residual may be y itself, not lie across it)
+    if (const int rc = ranges_apart("dropout", {range3("y", y, 1, 0, rows, y_stride, C, es)}, {{"rng", rng, 16}})) return rc;
     DropoutArgs a{};
     a.x = x; a.res = residual; a.y = y; a.rng = rng;
     a.n = rows * C; a.C = (unsigned)C;

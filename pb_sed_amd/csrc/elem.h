@@ -1,6 +1,9 @@
 // Element types of the sequence operators (causal_conv.hip, selective_scan.hip, layer_norm.hip, dropout.hip): activations are
 // float, bfloat16 or half in memory; every computation is float; one rounding (to nearest even) at the store.
 #pragma once
+#include <cstdint>
+#include <initializer_list>
+
 #include "common.h"
 
 namespace pbsed {
@@ -104,6 +107,31 @@ __device__ __forceinline__ void sum_partials(const float* ws, int P, long W, con
         }
     }
 }
+
+// Memory of an operand, first to last byte: what a launch writes must not be what it, or a launch behind it, still reads (or writes).
+struct Range {
+    const char* name;
+    const void* p;              // null: not given
+    long long bytes;
+};
+// rows of C elements of `es` bytes at strides over two axes
+inline Range range3(const char* name, const void* p, long long n0, long long s0, long long n1, long long s1, long long C, size_t es) {
+    return Range{name, p, ((n0 - 1) * s0 + (n1 - 1) * s1 + C) * (long long)es};
+}
+inline bool ranges_meet(const Range& a, const Range& b) {
+    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    return pa && pb && pa < pb + (uintptr_t)b.bytes && pb < pa + (uintptr_t)a.bytes;
+}
+inline int ranges_apart(const char* op, std::initializer_list<Range> written, std::initializer_list<Range> read) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        const Range* hit = nullptr;
+        for (auto o = w + 1; o != written.end() && !hit; ++o) hit = ranges_meet(*w, *o) ? &*o : nullptr;
+        for (auto r = read.begin(); r != read.end() && !hit; ++r) hit = ranges_meet(*w, *r) ? &*r : nullptr;
+        if (hit) { set_error("%s: %s overlaps %s", op, w->name, hit->name); return PBSED_E_ARG; }
+    }
+    return PBSED_OK;
+}
+inline size_t elem_size(int dtype) { return dtype == PBSED_DT_F32 ? 4 : 2; }
 
 }  // namespace pbsed
 

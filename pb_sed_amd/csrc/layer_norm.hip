@@ -332,6 +332,9 @@ extern "C" int pbsed_layer_norm_fwd(const void* x, const float* w, const float* 
                                     long long x_stride, float eps, int dtype, void* stream) {
     if (const int rc = norm_check("layer_norm_fwd", rows, C, x_stride, x_stride, dtype)) return rc;
     if (!x || !y) { set_error("layer_norm_fwd: null pointer"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);
+    if (const int rc = ranges_apart("layer_norm_fwd", {{"stats", stats, 8 * rows}, {"y", y, rows * C * (long long)es}},
+                                    {{"weight", w, 4 * C}, {"bias", b, 4 * C}, range3("x", x, 1, 0, rows, x_stride, C, es)})) return rc;
     NormArgs a{};
     a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats;
     a.rows = (int)rows; a.C = (int)C; a.xs = x_stride; a.eps = eps;
@@ -353,6 +356,11 @@ extern "C" int pbsed_layer_norm_bwd(const void* dy, const void* x, const float* 
         set_error("layer_norm_bwd: the weight gradients need a workspace of %lld floats, got %lld", pbsed_layer_norm_workspace(rows, C), ws_floats);
         return PBSED_E_ARG;
     }
+    const size_t es = elem_size(dtype);
+    if (const int rc = ranges_apart("layer_norm_bwd", {{"dweight", dw, 4 * C}, {"dbias", db, 4 * C}, {"dx", dx, rows * C * (long long)es},
+                                                       {"workspace", sums ? ws : nullptr, 4 * ws_floats}},
+                                    {{"weight", w, 4 * C}, {"stats", stats, 8 * rows}, range3("x", x, 1, 0, rows, x_stride, C, es),
+                                     range3("dy", dy, 1, 0, rows, dy_stride, C, es)})) return rc;
     NormArgs a{};
     a.x = x; a.dy = dy; a.w = w; a.y = dx; a.stats = const_cast<float*>(stats); a.ws = sums ? ws : nullptr;
     a.rows = (int)rows; a.C = (int)C; a.xs = x_stride; a.dys = dy_stride;

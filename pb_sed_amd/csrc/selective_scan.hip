@@ -1172,6 +1172,14 @@ extern "C" int pbsed_selective_scan_fwd(const void* u, const void* delta, const 
         return PBSED_E_ARG;
     }
     if ((uintptr_t)saved & 15) { set_error("selective_scan_fwd: saved states must be 16-byte aligned"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);
+    const long long states = 4ll * B * D * N;
+    auto act = [&](const char* name, const void* v, int k, int width) { return range3(name, v, T, strides[2 * k], B, strides[2 * k + 1], width, es); };
+    if (const int rc = ranges_apart("selective_scan_fwd", {{"y", y, (long long)T * B * D * (long long)es}, {"state_out", state_out, states}, {"saved", saved, 4 * p.saved},
+                                                           {"workspace", p.ws ? ws : nullptr, 4 * p.ws}},
+                                    {act("u", u, 0, D), act("delta", delta, 1, D), act("b", b, 2, N), act("c", c, 3, N), act("z", z, 4, D),
+                                     {"a_log", a_log, 4ll * D * N}, {"d", skip, 4ll * D}, {"delta_bias", delta_bias, 4ll * D}, {"seq_len", seq_len, 4ll * B},
+                                     {"state", state, states}})) return rc;
     ScanArgs a{};
     a.u = u; a.delta = delta; a.a_log = a_log; a.b = b; a.c = c; a.skip = skip; a.z = z; a.dbias = delta_bias; a.seq_len = seq_len;
     a.h0 = state; a.y = y; a.h_out = state_out; a.saved = saved;
@@ -1203,6 +1211,19 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
         set_error("selective_scan_bwd: needs a 16-byte aligned workspace of %lld floats (got %lld) and aligned saved states", p.ws, ws_floats);
         return PBSED_E_ARG;
     }
+    const size_t es = elem_size(dtype);
+    const long long states = 4ll * B * D * N, whole = (long long)T * B * D * (long long)es, bcs = (long long)T * B * N * (long long)es;
+    auto act = [&](const char* name, const void* v, int k, int width) { return range3(name, v, T, strides[2 * k], B, strides[2 * k + 1], width, es); };
+    const Range gate = act("dz", z ? dz : nullptr, 6, D);
+    if (const int rc = ranges_apart("selective_scan_bwd", {{"da_log", da_log, 4ll * D * N}, {"dd", dskip, 4ll * D}, {"ddelta_bias", ddelta_bias, 4ll * D},
+                                                           {"dstate", dstate, states}, {"du", du, whole}, {"ddelta", ddelta, whole}, {"db", db, bcs}, {"dc", dc, bcs},
+                                                           {"workspace", ws, 4 * p.ws}},
+                                    {gate, act("u", u, 0, D), act("delta", delta, 1, D), act("b", b, 2, N), act("c", c, 3, N), act("z", z, 4, D), act("dy", dy, 5, D),
+                                     {"a_log", a_log, 4ll * D * N}, {"d", skip, 4ll * D}, {"delta_bias", delta_bias, 4ll * D}, {"seq_len", seq_len, 4ll * B},
+                                     {"saved", saved, 4 * p.saved}, {"dstate_out", dstate_out, states}})) return rc;
+    if (const int rc = ranges_apart("selective_scan_bwd", {gate}, {{"a_log", a_log, 4ll * D * N}, {"d", skip, 4ll * D}, {"delta_bias", delta_bias, 4ll * D},
+                                                                   {"seq_len", seq_len, 4ll * B}, {"saved", saved, 4 * p.saved}, {"dstate_out", dstate_out, states}}))
+        return rc;
     ScanArgs a{};
     a.dy = dy; a.u = u; a.delta = delta; a.a_log = a_log; a.b = b; a.c = c; a.skip = skip; a.z = z; a.dbias = delta_bias; a.seq_len = seq_len;
     a.saved = const_cast<float*>(saved); a.dh_out = dstate_out; a.du = du; a.ddelta = ddelta; a.db = db; a.dc = dc; a.dz = dz; a.dh0 = dstate;
@@ -1231,6 +1252,13 @@ extern "C" int pbsed_selective_scan_step(const void* u, const void* delta, const
                                          const long long* strides /*host*/, int B, int D, int N, int softplus, int dtype, void* stream) {
     if (const int rc = scan_check("selective_scan_step", 1, B, D, N, dtype)) return rc;
     if (!u || !delta || !a_log || !b || !c || !state || !state_out || !y || !strides) { set_error("selective_scan_step: null pointer"); return PBSED_E_ARG; }
+    const size_t es = elem_size(dtype);
+    const long long states = 4ll * B * D * N;
+    auto act = [&](const char* name, const void* v, int k, int width) { return range3(name, v, 1, 0, B, strides[k], width, es); };
+    if (const int rc = ranges_apart("selective_scan_step", {{"y", y, (long long)B * D * (long long)es}, {"state_out", state_out, states}},
+                                    {act("u", u, 0, D), act("delta", delta, 1, D), act("b", b, 2, N), act("c", c, 3, N), act("z", z, 4, D),
+                                     {"a_log", a_log, 4ll * D * N}, {"d", skip, 4ll * D}, {"delta_bias", delta_bias, 4ll * D},
+                                     {"state", state == state_out ? nullptr : state, states}})) return rc;
     ScanArgs a{};
     a.u = u; a.delta = delta; a.a_log = a_log; a.b = b; a.c = c; a.skip = skip; a.z = z; a.dbias = delta_bias; a.h0 = state; a.h_out = state_out; a.y = y;
     a.ub = strides[0]; a.eb = strides[1]; a.bb = strides[2]; a.cb = strides[3]; a.zb = strides[4];

@@ -160,3 +160,52 @@ def test_infinities_without_the_skip_weight(dev):                     # noqa: F8
     for f in range(10):
         one = ops.selective_scan_step(u[f], delta[f], a_log, b[f], c[f], h, z=z[f])
         assert torch.equal(torch.isposinf(one.cpu()), torch.isposinf(y[f].cpu())) and not torch.isnan(one).any(), f
+
+
+# ------------------------------------------------------------------------------------------------ memory that is read and written
+def test_outputs_over_operands_are_refused(dev):                      # noqa: F811
+    """What a launch writes must not be what it still reads, nor another output: refused before anything is launched."""
+    from pb_sed_amd import ops
+    t, b, d, k, n = 4, 2, 6, 4, 5
+    f = lambda *s, dtype=F32: torch.zeros(*s, dtype=dtype, device=dev)     # noqa: E731
+    over = lambda v, *s, off=0: v.flatten()[off:off + int(np.prod(s))].view(s)   # noqa: E731
+    arena = f(600)
+    x, w, bias, cs = f(t, b, d), f(d, k), f(d), f(b, k - 1, d)
+    u, al, bc, h = f(t, b, d), f(d, n), f(t, b, n), f(b, d, n)
+    saved = ops.selective_scan_fwd(u, u, al, bc, bc, save=True)[2]
+    stats = ops.layer_norm_fwd(x, save=True)[1]
+    conv_bwd = lambda **o: ops.causal_conv_bwd(o.pop('dy', x.clone()), o.pop('x', x), o.pop('w', w), o.pop('bias', bias), **o)        # noqa: E731
+    scan_bwd = lambda **o: ops.selective_scan_bwd(**{**dict(dy=u, u=u, delta=u, a_log=al, b=bc, c=bc, saved=saved), **o})             # noqa: E731
+    step = lambda **o: ops.selective_scan_step(**{**dict(u=u[0], delta=u[0], a_log=al, b=bc[0], c=bc[0], state=h), **o})              # noqa: E731
+    norm_bwd = lambda **o: ops.layer_norm_bwd(x, o.pop('x', x), o.pop('w', bias), o.pop('stats', stats), **o)                         # noqa: E731
+    state, near, head, frame = over(arena, b, k - 1, d), over(arena, b, d, off=30), over(arena, d, off=35), over(arena, t, b, d, off=3)
+    big = over(arena, b, d, n)
+    shared = over(saved, t, b, d)
+    refused = [
+        lambda: ops.causal_conv_step(near, w, bias, state), lambda: ops.causal_conv_step(near, w, bias, cs, state_out=state),
+        lambda: ops.causal_conv_step(x[0], over(arena, d, k, off=20), bias, cs, state_out=state), lambda: ops.causal_conv_step(x[0], w, head, cs, state_out=state),
+        lambda: ops.causal_conv_step(x[0], w, head, state),
+        lambda: conv_bwd(w=over(arena, d, k), dx=frame), lambda: conv_bwd(bias=over(arena, d, off=50), dx=frame), lambda: conv_bwd(state=state, dx=frame),
+        lambda: conv_bwd(dweight=over(arena, d, k), dx=frame), lambda: conv_bwd(dbias=over(arena, d, off=50), dx=frame),
+        lambda: conv_bwd(dweight=w), lambda: conv_bwd(dbias=bias), lambda: conv_bwd(x=frame, dweight=over(arena, d, k)), lambda: conv_bwd(dy=frame, dbias=head),
+        lambda: conv_bwd(state=state, dweight=over(arena, d, k)), lambda: conv_bwd(dstate_out=state, dweight=over(arena, d, k)),
+        lambda: scan_bwd(z=u, dz=shared), lambda: scan_bwd(z=u, dz=frame, dstate_out=big), lambda: scan_bwd(z=u, dz=frame, da_log=over(arena, d, n)),
+        lambda: scan_bwd(z=u, dz=frame, dd=head), lambda: scan_bwd(z=u, dz=frame, ddelta_bias=head), lambda: scan_bwd(z=u, dz=frame, a_log=over(arena, d, n)),
+        lambda: scan_bwd(da_log=al), lambda: scan_bwd(dd=over(u, d)), lambda: scan_bwd(ddelta_bias=over(saved, d)), lambda: scan_bwd(d=head, dd=head),
+        lambda: scan_bwd(da_log=over(bc, d, n)), lambda: scan_bwd(dstate_out=big, da_log=over(arena, d, n)),
+        lambda: step(state=big, u=near), lambda: step(state_out=big, delta=near), lambda: step(state_out=big, b=over(arena, b, n, off=7)),
+        lambda: step(state_out=big, c=over(arena, b, n, off=7)), lambda: step(state_out=big, z=near), lambda: step(state_out=big, a_log=over(arena, d, n, off=9)),
+        lambda: step(state_out=big, d=head), lambda: step(state_out=big, delta_bias=head), lambda: step(state=big, a_log=over(arena, d, n, off=9)),
+        lambda: norm_bwd(dweight=bias), lambda: norm_bwd(dbias=over(x, d)), lambda: norm_bwd(dbias=over(stats, d)),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises((ValueError, RuntimeError), match='overlaps'):
+            call()
+            raise AssertionError(f'call {i} was accepted')
+    # neighbours in one buffer are no overlap
+    ops.causal_conv_step(over(arena, b, d, off=36), w, over(arena, d, off=48), state)
+    ops.causal_conv_bwd(x.clone(), x, w, bias, dweight=over(arena, d, k), dbias=over(arena, d, off=24), dx=over(arena, t, b, d, off=30))
+    step(state=over(arena, b, d, n), u=over(arena, b, d, off=60), a_log=over(arena, d, n, off=72))
+    wide = f(t, b, 2 * d)
+    ops.causal_conv_bwd(wide[..., d:], x, w, bias, dx=wide[..., :d])
+    scan_bwd(dy=wide[..., d:], z=u, dz=wide[..., :d])
