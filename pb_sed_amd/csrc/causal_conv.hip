@@ -319,15 +319,12 @@ static void cconv_launch2(const CConvArgs& a, int K, bool bwd, hipStream_t s) {
         default: return cconv_launch3<S, V, 8>(a, bwd, s);
     }
 }
+static int cconv_width(int D) { return D >= 4 ? 4 : 1; }            // channels per thread
 template <class S>
 static int cconv_launch(CConvArgs& a, int K, bool bwd, hipStream_t s) {
-    const int full = 4, v = a.D >= full ? full : 1;
+    const int v = cconv_width(a.D);
     a.ts = cconv_ts(a.T, a.B, a.D, v);
     a.nrun = (a.T + a.ts - 1) / a.ts;
-    if (!bwd && (long long)a.B * a.nrun * ((a.D + 64 * v - 1) / (64 * v)) > 4 * CC_BLOCKS) {
-        set_error("causal_conv_fwd: T = %d, B = %d, D = %d need more than %lld blocks", a.T, a.B, a.D, CC_BLOCKS);
-        return PBSED_E_UNSUPPORTED;
-    }
     if (v == 1) cconv_launch2<S, 1>(a, K, bwd, s);
     else cconv_launch2<S, 4>(a, K, bwd, s);
     return check_launch(bwd ? "causal_conv_bwd" : "causal_conv_fwd");
@@ -361,6 +358,11 @@ extern "C" int pbsed_causal_conv_fwd(const void* x, const float* w, const float*
                                      int silu, int reverse, int dtype, void* stream) {
     if (const int rc = cconv_check("causal_conv_fwd", T, B, D, K, dtype)) return rc;
     if (!x || !w || !y) { set_error("causal_conv_fwd: null pointer"); return PBSED_E_ARG; }
+    const int v = cconv_width(D), ts = cconv_ts(T, B, D, v);
+    if ((long long)B * ((T + ts - 1) / ts) * ((D + 64 * v - 1) / (64 * v)) > 4 * CC_BLOCKS) {
+        set_error("causal_conv_fwd: T = %d, B = %d, D = %d need more than %lld blocks", T, B, D, CC_BLOCKS);
+        return PBSED_E_UNSUPPORTED;
+    }
     const size_t es = elem_size(dtype);
     const long long whole = (long long)T * B * D * es, states = (long long)B * (K - 1) * D * es;
     if (const int rc = ranges_apart("causal_conv_fwd", {{"y", y, whole}, {"state_out", state_out, states}},
@@ -419,13 +421,13 @@ extern "C" int pbsed_causal_conv_step(const void* x, const float* w, const float
                                       int D, int K, long long x_stride_b, int silu, int dtype, void* stream) {
     if (const int rc = cconv_check("causal_conv_step", 1, B, D, K, dtype)) return rc;
     if (!x || !w || !state || !state_out || !y) { set_error("causal_conv_step: null pointer"); return PBSED_E_ARG; }
+    const long long grid = ((long long)B * D + 255) / 256;
+    if (grid > CC_BLOCKS) { set_error("causal_conv_step: B = %d, D = %d need more than %lld blocks", B, D, CC_BLOCKS); return PBSED_E_UNSUPPORTED; }
     const size_t es = elem_size(dtype);
     const long long states = (long long)B * (K - 1) * D * es;
     if (const int rc = ranges_apart("causal_conv_step", {{"y", y, (long long)B * D * (long long)es}, {"state_out", state_out, states}},
                                     {range3("x", x, 1, 0, B, x_stride_b, D, es), {"weight", w, 4ll * D * K}, {"bias", bias, 4ll * D},
                                      {"state", state == state_out ? nullptr : state, states}})) return rc;
-    const long long grid = ((long long)B * D + 255) / 256;
-    if (grid > CC_BLOCKS) { set_error("causal_conv_step: B = %d, D = %d need more than %lld blocks", B, D, CC_BLOCKS); return PBSED_E_UNSUPPORTED; }
     PBSED_ELEM(dtype, hipLaunchKernelGGL(causal_conv_step_kernel<S>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, static_cast<const S*>(x),
                                          x_stride_b, w, bias, static_cast<const S*>(state), static_cast<S*>(state_out), static_cast<S*>(y),
                                          B, D, K, silu));

@@ -1078,7 +1078,7 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
 
 static int scan_check(const char* name, int T, int B, int D, int N, int dtype) {
     if (dtype < 0 || dtype > 2) { set_error("%s: element type %d", name, dtype); return PBSED_E_ARG; }
-    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 24) || N < 1 || N > 64 || (long long)D * (N + 2) >= (1 << 26)) {       // (64 parameter sums per 1024 threads, < 2^32 threads)
+    if (T < 1 || T > (1 << 28) || B < 1 || B > 65535 || D < 1 || D > (1 << 24) || N < 1 || N > 64 || (long long)D * (N + 2) >= (1 << 26)) {
         set_error("%s: T = %d, B = %d, D = %d, N = %d (T <= 2^28, B <= 65535, N <= 64, D (N + 2) < 2^26)", name, T, B, D, N);
         return PBSED_E_ARG;
     }
@@ -1207,6 +1207,14 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
     }
     if (const int rc = scan_strides("selective_scan_bwd", strides, 7, B, D)) return rc;
     const ScanPlan p = scan_plan(T, B, D, N, true);
+    // the last launch: blocks for the parameters' sums, then blocks for dB and dC
+    const long W = (long)D * (N + 2);
+    const long long n = (long long)T * B * 2 * p.np, most = 2ll * device_cus(), need = (n + SUM_THREADS - 1) / SUM_THREADS;
+    const long long nbc = need < most ? need : most, nsum = da_log || dskip || ddelta_bias ? (W + 15) / 16 : 0;
+    if ((nsum + nbc) * SUM_THREADS >= 1ll << 32) {
+        set_error("selective_scan_bwd: D = %d, N = %d: the sums need %lld blocks of %d threads", D, N, nsum + nbc, SUM_THREADS);
+        return PBSED_E_UNSUPPORTED;
+    }
     if (!ws || ws_floats < p.ws || ((uintptr_t)ws & 15) || ((uintptr_t)saved & 15)) {
         set_error("selective_scan_bwd: needs a 16-byte aligned workspace of %lld floats (got %lld) and aligned saved states", p.ws, ws_floats);
         return PBSED_E_ARG;
@@ -1228,7 +1236,7 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
     a.dy = dy; a.u = u; a.delta = delta; a.a_log = a_log; a.b = b; a.c = c; a.skip = skip; a.z = z; a.dbias = delta_bias; a.seq_len = seq_len;
     a.saved = const_cast<float*>(saved); a.dh_out = dstate_out; a.du = du; a.ddelta = ddelta; a.db = db; a.dc = dc; a.dz = dz; a.dh0 = dstate;
     a.runs = ws; a.runs_dt = ws + p.o_dt; a.bc = ws + p.o_bc;
-    a.sums = da_log || dskip || ddelta_bias ? ws + p.o_sums : nullptr;
+    a.sums = nsum ? ws + p.o_sums : nullptr;
     a.ut = strides[0]; a.ub = strides[1]; a.et = strides[2]; a.eb = strides[3]; a.bt = strides[4]; a.bb = strides[5];
     a.ct = strides[6]; a.cb = strides[7]; a.zt = strides[8]; a.zb = strides[9]; a.gt = strides[10]; a.gb = strides[11];
     a.dzt = strides[12]; a.dzb = strides[13];
@@ -1237,12 +1245,9 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
     int rc = PBSED_OK;
     PBSED_SCAN(scan_bwd_launch);
     if (rc) return rc;
-    const long W = (long)D * (N + 2);
     const SumSegs sg{{da_log, dskip, ddelta_bias}, {D * N, D * (N + 1), D * (N + 2)}};
-    const long long n = (long long)T * B * 2 * p.np, most = 2ll * device_cus(), need = (n + SUM_THREADS - 1) / SUM_THREADS;
-    const unsigned nbc = (unsigned)(need < most ? need : most), nsum = a.sums ? (unsigned)((W + 15) / 16) : 0;
-    PBSED_ELEM(dtype, hipLaunchKernelGGL(scan_sum_kernel<S>, dim3(nsum + nbc), dim3(SUM_THREADS), 0, s, a.bc, static_cast<S*>(db), static_cast<S*>(dc),
-                                         p.blocks, (long long)T * B, N, p.np, a.sums, B * p.nrun, W, nsum, sg));
+    PBSED_ELEM(dtype, hipLaunchKernelGGL(scan_sum_kernel<S>, dim3((unsigned)(nsum + nbc)), dim3(SUM_THREADS), 0, s, a.bc, static_cast<S*>(db), static_cast<S*>(dc),
+                                         p.blocks, (long long)T * B, N, p.np, a.sums, B * p.nrun, W, (unsigned)nsum, sg));
     return check_launch("selective_scan_bwd sums");
 }
 

@@ -209,3 +209,24 @@ def test_outputs_over_operands_are_refused(dev):                      # noqa: F8
     wide = f(t, b, 2 * d)
     ops.causal_conv_bwd(wide[..., d:], x, w, bias, dx=wide[..., :d])
     scan_bwd(dy=wide[..., d:], z=u, dz=wide[..., :d])
+
+
+def test_launches_beyond_the_grid_are_named():
+    """Refused for their size (pointers, never read, would be refused as overlapping behind that): the message names the blocks or the
+    limit.  The scan's last launch holds blocks for the parameters' sums and for dB, dC: together less than 2^32 threads."""
+    import ctypes
+    from pb_sed_amd import _lib
+    lib = _lib.lib()
+    p, big, strides = 1 << 20, 1 << 22, (ctypes.c_longlong * 16)()
+    scan = lambda d, n, sums: lib.pbsed_selective_scan_bwd(p, p, p, p, p, p, None, None, None, None, p, None, p, p, p, p, None, None, p if sums else None, None, None,  # noqa: E731
+                                                           p, 1 << 50, strides, 300, 1, d, n, 1, 0, 0, None)
+    calls = [
+        (lambda: lib.pbsed_causal_conv_fwd(p, p, None, None, None, p, None, 1, 65535, big, 4, 65535 * big, big, 1, 0, 0, None), 'blocks'),
+        (lambda: lib.pbsed_causal_conv_step(p, p, None, p, p, p, 65535, big, 4, big, 1, 0, None), 'blocks'),
+        (lambda: scan(8388600, 6, True), 'blocks'),            # 4194300 blocks of sums, at least 5 of dB and dC
+        (lambda: scan(8388600, 6, False), 'overlaps'),
+        (lambda: scan(8388400, 6, False), 'overlaps'),
+        (lambda: scan(1 << 18, 254, True), 'N <= 64'),
+    ]
+    for i, (call, word) in enumerate(calls):
+        assert call() < 0 and word in lib.pbsed_last_error().decode(), (i, lib.pbsed_last_error())
