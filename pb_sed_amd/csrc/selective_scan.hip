@@ -36,12 +36,14 @@ struct ScanArgs {
     float *runs, *runs_dt;                             // [nrun][B][D][NP] end states, [nrun][B][D] sums of D
     float* bc;                                         // backward: [channel blocks][T][B][2 NP] partial sums of dB | dC
     float* sums;                                       // backward: [B nrun][D N + 2 D] partial sums of da_log | dskip | ddelta_bias
+    double* acc;                                       // backward: [B nrun][channel blocks][NS + 2][256] a thread's sums so far, or null
     long long ut, ub, et, eb, bt, bb, ct, cb, zt, zb, gt, gb, dzt, dzb;      // strides over frames and clips (elements)
     int T, B, D, N, reverse, softplus, nrun, run;      // run: frames per run, a number of tiles
     int folded;                                        // runs hold the states in front of the runs (a scan_runs kernel has been there)
 };
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr int SC_FLUSH = 512;                          // frames whose sums for the parameters are added up in float
 constexpr int SC_SAVE = 16;                            // frames between saved states; also the tile of the backward kernel
 
 template <int CTRL> __device__ __forceinline__ float dpp_lane(float v) {        // every lane has a source: folds into the addition
@@ -308,6 +310,13 @@ template <int NS> __device__ __forceinline__ void arrived(float (&v)[NS]) {     
     for (int j = 0; j < NS; ++j) asm volatile("" : "+v"(v[j]));
 #endif
 }
+// v, for an address that is worked out where it is used: a rare branch's, which would hold registers through the whole loop otherwise
+__device__ __forceinline__ int here(int v) {
+#ifndef HIP_EMU
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
+}
 // What lanes of a wave leave in LDS for one another: the wave's LDS accesses keep their order, the compiler must too.
 __device__ __forceinline__ void wave_handover() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -451,7 +460,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
             for (int i = 0; i < 4; ++i) row_store<S>(0.f, rows_at(y), SC_OUT, 4 * i);
     }
     for (; t0 < stop; t0 += TT, buf ^= 1) {
-        float uc[4], gate[4], D4[4], U4[4], e4[4], z4[4];
+        float uc[4], gate[4], D4[4], U4[4], e4[4], z4[4], dtile = 0.f;
         values_of<S>(re, e4);
         values_of<S>(ru, uc);
         values_of<S>(rz, z4);
@@ -498,7 +507,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
                     if (MIX && j) h[j] = nq * NS + j < a.N ? h[j] : 0.f;
                     if constexpr (!SUMMARY) y4[i] = j ? fmaf(g.Cv[i].v[j], h[j], y4[i]) : g.Cv[i].v[j] * h[j];
                 }
-                if (SUMMARY) dsum += at(g.D, i);
+                if (SUMMARY) dtile += at(g.D, i);
             }
             if constexpr (!SUMMARY) {
                 lanes_sum4<LN, 1>(y4);
@@ -510,7 +519,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
             }
             if (q + 1 < TT / 4) g = next;
         }
-        if (SUMMARY) continue;
+        if (SUMMARY) {
+            dsum += dtile;
+            continue;
+        }
         __syncthreads();
         float o[4];
         load_pack<float, 4>(&sD[buf][sch * LD + sq * 4], o);
@@ -577,7 +589,7 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
     };
     if (t0 >= p0) fetch(len - t0);
     for (; t0 >= p0; t0 -= TT, buf ^= 1) {
-        float D4[4], G4[4], e4[4], z4[4];
+        float D4[4], G4[4], e4[4], z4[4], dtile = 0.f;
         values_of<S>(re, e4);
         values_of<S>(rz, z4);
         values_of<S>(rg, G4);
@@ -611,10 +623,11 @@ __global__ __launch_bounds__(256) void scan_bwd_summary_kernel(ScanArgs a) {
                     r[j] = fmaf(gr.B[i].v[j], at(gr.U, i), r[j]) * ex[i][j];
                     if (MIX && j) r[j] = nq * NS + j < a.N ? r[j] : 0.f;
                 }
-                dsum += at(gr.D, i);
+                dtile += at(gr.D, i);
             }
             if (q) gr = next;
         }
+        dsum += dtile;
     }
     if (d < a.D) {
         const long long at_ = ((long long)c * a.B + b) * a.D + d;
@@ -711,6 +724,7 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
     const float bias = chan && a.dbias ? a.dbias[sd] : 0.f, skip = chan && a.skip ? a.skip[sd] : 0.f;
     const unsigned skip_mask = a.skip ? ~0u : 0u;
     float dskip = 0.f, dbias = 0.f;
+    bool flushed = false;
     float A2[NS], A[NS], r[NS] = {}, da[NS] = {};
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
@@ -763,9 +777,11 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
         oc.put(lds_bc + L::bc, rc);
     }
     __syncthreads();
-    for (int buf = 0; t0 >= p0; t0 -= TT, buf ^= 1) {
+    for (int buf = 0; t0 >= p0;) {
+    const int turn = max(p0, t0 / SC_FLUSH * SC_FLUSH);
+    for (; t0 >= turn; t0 -= TT, buf ^= 1) {
         float *sB = lds_bc + buf * 2 * L::bc, *sC = sB + L::bc, *sP = lds_part + (L::parts > 1 ? buf * L::part : 0);
-        float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F];
+        float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F], tile_skip = 0.f;
         values_of<S>(ru, u4);
         values_of<S>(re, e4);
         values_of<S>(rz, z4);
@@ -788,7 +804,8 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
                 G4[i] = G4[i] * (z4[i] * sg);
             }
 #pragma unroll
-        for (int i = 0; i < F; ++i) dskip = fmaf(G4[i], u4[i], dskip);
+        for (int i = 0; i < F; ++i) tile_skip = fmaf(G4[i], u4[i], tile_skip);
+        dskip += tile_skip;
         store_pack<float, F>(sD + sch * LD + sq * F, D4);
         store_pack<float, F>(sU + sch * LD + sq * F, U4);
         store_pack<float, F>(sG + sch * LD + sq * F, G4);
@@ -882,7 +899,7 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
             }
         }
 #pragma unroll
-        for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (sums over a tile first: long clips keep their digits)
+        for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (a tile's sum first, 32 tiles in float, the rest in double)
         if (t0 - TT >= p0) {                                     // B and C are the block's: the next tile's go where the last one's were
             ob.put(lds_bc + (buf ^ 1) * 2 * L::bc, rb);
             oc.put(lds_bc + (buf ^ 1) * 2 * L::bc + L::bc, rc);
@@ -918,8 +935,28 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
         du += adv * row; de += adv * row; dz += adv * a.dzt; bc += adv * a.B * 2 * NP;
         if (L::parts == 1) __syncthreads();
     }
+    if (a.acc && t0 >= p0) {                                     // long runs: what has been added up so far moves to the thread's doubles
+        double* acc = a.acc + ((((long long)c * a.B + b) * gridDim.x + blk.x) * (NS + 2)) * 256 + here(tid);
+        auto move = [&](int k, float& v) {
+            acc[k * 256] = (flushed ? acc[k * 256] : 0.) + (double)v;
+            v = 0.f;
+        };
+#pragma unroll
+        for (int j = 0; j < NS; ++j) move(j, da[j]);
+        move(NS, dskip);
+        move(NS + 1, dbias);
+        flushed = true;
+    }
+    }
     if (a.dh0 && d < a.D && c == 0) store_states<NS>(a.dh0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
     if (!a.sums) return;
+    if (flushed) {
+        const double* acc = a.acc + ((((long long)c * a.B + b) * gridDim.x + blk.x) * (NS + 2)) * 256 + tid;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) da[j] = (float)(acc[j * 256] + (double)da[j]);
+        dskip = (float)(acc[NS * 256] + (double)dskip);
+        dbias = (float)(acc[(NS + 1) * 256] + (double)dbias);
+    }
     float* out = a.sums + ((long long)c * a.B + b) * ((long long)a.D * (a.N + 2));
     if (d < a.D) {
 #pragma unroll
@@ -1039,7 +1076,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 struct ScanPlan {
     int ln, ns, np, cb, blocks, nrun, run;               // blocks: channel blocks
     long long saved, ws;                                 // floats
-    long long o_dt, o_bc, o_sums;                        // offsets in the workspace
+    long long o_dt, o_bc, o_sums, o_acc;                 // offsets in the workspace
 };
 // Frames are cut into runs where channel blocks x clips leave CUs with hardly more than one block: a lone block per CU is bound by the
 // latency of its chain, and a cut costs the first launch (about 0.7 of the main one's work).  Up to SC_FOLD runs the main launch folds
@@ -1072,7 +1109,8 @@ static ScanPlan scan_plan(int T, int B, int D, int N, bool bwd) {
     p.o_dt = runs * p.np;
     p.o_bc = (p.o_dt + runs + 3) & ~3ll;
     p.o_sums = p.o_bc + (bwd ? (long long)p.blocks * T * B * 2 * p.np : 0);
-    p.ws = p.o_sums + (bwd ? (long long)p.nrun * B * D * (N + 2) : 0);
+    p.o_acc = (p.o_sums + (bwd ? (long long)p.nrun * B * D * (N + 2) : 0) + 3) & ~3ll;
+    p.ws = p.o_acc + (bwd && p.run > SC_FLUSH ? 2ll * p.nrun * B * p.blocks * (p.ns + 2) * 256 : 0);       // (16-byte offsets: doubles)
     return p;
 }
 
@@ -1237,6 +1275,7 @@ extern "C" int pbsed_selective_scan_bwd(const void* dy, const void* u, const voi
     a.saved = const_cast<float*>(saved); a.dh_out = dstate_out; a.du = du; a.ddelta = ddelta; a.db = db; a.dc = dc; a.dz = dz; a.dh0 = dstate;
     a.runs = ws; a.runs_dt = ws + p.o_dt; a.bc = ws + p.o_bc;
     a.sums = nsum ? ws + p.o_sums : nullptr;
+    a.acc = nsum && p.run > SC_FLUSH ? reinterpret_cast<double*>(ws + p.o_acc) : nullptr;
     a.ut = strides[0]; a.ub = strides[1]; a.et = strides[2]; a.eb = strides[3]; a.bt = strides[4]; a.bb = strides[5];
     a.ct = strides[6]; a.cb = strides[7]; a.zt = strides[8]; a.zb = strides[9]; a.gt = strides[10]; a.gb = strides[11];
     a.dzt = strides[12]; a.dzb = strides[13];

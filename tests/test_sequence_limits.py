@@ -230,3 +230,39 @@ def test_launches_beyond_the_grid_are_named():
     ]
     for i, (call, word) in enumerate(calls):
         assert call() < 0 and word in lib.pbsed_last_error().decode(), (i, lib.pbsed_last_error())
+
+
+# ------------------------------------------------------------------------------------------------ sums over long axes
+def test_sums_of_long_uncut_scans_keep_their_digits(dev):             # noqa: F811
+    """Terms of one sign over many frames of a scan that is not cut into runs (clips and channels fill the device): the bound counts a tile's
+    terms, the 32 tiles that are added in float and the groups of frames of a block - 16 + 32 + 16 + 4 roundings - not the frames."""
+    from pb_sed_amd import ops
+    t, b = (3500, 10) if dev == 'cpu' else (20000, 300)
+    d, n = 2, 2
+    # 4/3: every addition to a sum is off by a third of its last place, in one direction while the sum's exponent lasts
+    u, dy, delta = torch.full((t, b, d), 4 / 3), torch.ones(t, b, d), torch.full((t, b, d), .7)
+    bm, cm = torch.ones(t, b, n), torch.ones(t, b, n)
+    a_log, skip = torch.zeros(d, n), torch.ones(d)
+    x = [v.to(dev) for v in (u, delta, a_log, bm, cm)]
+    _, _, saved = ops.selective_scan_fwd(*x, d=skip.to(dev), save=True)
+    da, dd, db = torch.zeros(d, n, device=dev), torch.zeros(d, device=dev), torch.zeros(d, device=dev)
+    ddelta = ops.selective_scan_bwd(dy.to(dev), *x, saved, d=skip.to(dev), da_log=da, dd=dd, ddelta_bias=db)[1]
+    k = 16 + 32 + 16 + 4
+    want = b * (dy[:, 0].double() * u[:, 0].double()).sum(0)
+    check(dd, want, want, k, 'dd')
+    terms = ddelta.double().cpu()
+    check(db, terms.sum((0, 1)), terms.abs().sum((0, 1)), k, 'ddelta_bias')      # (the launch's own float terms)
+    # da_log against the recurrence in float64: D, exp, h and r carry some 30 roundings of a frame each, for a factor of 0.27
+    # and less per frame (1 / (1 - 0.27)): 2 x 42 more
+    step = torch.nn.functional.softplus(delta[:, 0].double())[..., None]
+    decay, drive = torch.exp(-step), step * (u[:, 0, :, None] * bm[:, 0, None]).double()
+    h, past = torch.zeros(d, n, dtype=torch.float64), []
+    for f in range(t):
+        past.append(h)
+        h = decay[f] * h + drive[f]
+    r, want = torch.zeros(d, n, dtype=torch.float64), torch.zeros(d, n, dtype=torch.float64)
+    for f in reversed(range(t)):
+        r = r + dy[f, 0, :, None].double() * cm[f, 0, None].double()
+        want -= r * decay[f] * past[f] * step[f]
+        r = r * decay[f]
+    check(da, b * want, b * want.abs(), k + 2 * 42, 'da_log')
