@@ -177,9 +177,9 @@ __device__ __forceinline__ void fold_runs(const ScanArgs& a, int c, int from, in
         for (int j = 0; j < NS; ++j) h[j] = fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), h[j], s[j]);
     }
 }
-// Many runs (up to 256) of steps that softplus made (factors up to one): their end states become the states in front of them, in place.  A lane owns one state; wave w of a block's 16
-// takes runs 16 w .. 16 w + 15 of the order, holds them in registers, and learns through LDS what the waves in front of it add up to.
-// back: from the last run to the first, starting from dh_out.
+// Many runs (up to 256) of steps that softplus made (factors up to one): their end states become the states in front of them, in place.
+// A lane owns one state; wave w of a block's 16 takes runs 16 w .. 16 w + 15 of the order, holds them in registers, and learns through
+// LDS what the waves in front of it add up to.  back: from the last run to the first, starting from dh_out.
 __global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int back) {
     __shared__ float ss[16][64], sp[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -687,7 +687,8 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
     using BC = StateRows<S, TT, NP>;
     static_assert(F >= 1 && NP2 >= 1 && L::rows >= 256, "a tile has work for every thread");
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *lds_bc = sG + L::rows, *nothing = lds_bc + 4 * L::bc, *lds_part = nothing + L::bc;     // [2][B | C], [parts][4][TT][2 NP]
+    float *sD = smem, *sU = sD + L::rows, *sG = sU + L::rows, *lds_bc = sG + L::rows, *nothing = lds_bc + 4 * L::bc;      // [2][B | C]
+    float* lds_part = nothing + L::bc;                           // [parts][4][TT][2 NP]
     Pack<float, F>* keep = reinterpret_cast<Pack<float, F>*>(lds_part + L::parts * L::part) + threadIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nq = lane % LN;
     constexpr int WC = 64 / LN;                                  // channels of a wave: it stages them for itself
@@ -778,175 +779,175 @@ __global__ __launch_bounds__(256, NS > 2 || LN == 4 ? 2 : 3) void scan_bwd_kerne
     }
     __syncthreads();
     for (int buf = 0; t0 >= p0;) {
-    const int turn = max(p0, t0 / SC_FLUSH * SC_FLUSH);
-    for (; t0 >= turn; t0 -= TT, buf ^= 1) {
-        float *sB = lds_bc + buf * 2 * L::bc, *sC = sB + L::bc, *sP = lds_part + (L::parts > 1 ? buf * L::part : 0);
-        float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F], tile_skip = 0.f;
-        values_of<S>(ru, u4);
-        values_of<S>(re, e4);
-        values_of<S>(rz, z4);
-        values_of<S>(rg, G4);
-        steps_of<F>(a, e4, bias, sq * F, len - t0, D4);
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            S4[i] = fast_sigmoid(e4[i] + bias);
-            U4[i] = D4[i] * u4[i];
-            Z4[i] = 0.f;
-        }
-        if (!a.softplus)
-#pragma unroll
-            for (int i = 0; i < F; ++i) S4[i] = 1.f;
-        if (a.z)
+        const int turn = max(p0, t0 / SC_FLUSH * SC_FLUSH);
+        for (; t0 >= turn; t0 -= TT, buf ^= 1) {
+            float *sB = lds_bc + buf * 2 * L::bc, *sC = sB + L::bc, *sP = lds_part + (L::parts > 1 ? buf * L::part : 0);
+            float D4[F], U4[F], S4[F], G4[F], Z4[F], u4[F], e4[F], z4[F], tile_skip = 0.f;
+            values_of<S>(ru, u4);
+            values_of<S>(re, e4);
+            values_of<S>(rz, z4);
+            values_of<S>(rg, G4);
+            steps_of<F>(a, e4, bias, sq * F, len - t0, D4);
 #pragma unroll
             for (int i = 0; i < F; ++i) {
-                const float sg = fast_sigmoid(z4[i]);
-                Z4[i] = G4[i] * (sg * fmaf(z4[i], 1.f - sg, 1.f));
-                G4[i] = G4[i] * (z4[i] * sg);
+                S4[i] = fast_sigmoid(e4[i] + bias);
+                U4[i] = D4[i] * u4[i];
+                Z4[i] = 0.f;
             }
+            if (!a.softplus)
 #pragma unroll
-        for (int i = 0; i < F; ++i) tile_skip = fmaf(G4[i], u4[i], tile_skip);
-        dskip += tile_skip;
-        store_pack<float, F>(sD + sch * LD + sq * F, D4);
-        store_pack<float, F>(sU + sch * LD + sq * F, U4);
-        store_pack<float, F>(sG + sch * LD + sq * F, G4);
-        store_pack<float, F>(keep[0].v, D4);
-        store_pack<float, F>(keep[256].v, u4);
-        store_pack<float, F>(keep[512].v, S4);
-        store_pack<float, F>(keep[768].v, G4);
-        store_pack<float, F>(keep[1024].v, Z4);
-        float h[NS];
+                for (int i = 0; i < F; ++i) S4[i] = 1.f;
+            if (a.z)
 #pragma unroll
-        for (int j = 0; j < NS; ++j) h[j] = rh[j];
-        wave_handover();
-        if (t0 - TT >= p0) fetch(len - t0 + TT);
-        const float *rowB = bc0 + buf * bc_buf, *rowC = rowB + bc_c;
-        float *outD = sD + ch * LD, *outU = outD + L::rows, *outG = outU + L::rows;       // where the sums over the channel's states go
-        float ex[TT][NS], hs[TT][NS], h0[NS];                    // hs[t]: the state behind frame t
-#pragma unroll
-        for (int j = 0; j < NS; ++j) h0[j] = h[j];
-        ScanGroup<NS, false> gr;
-        gr.template load<NP>(rowD, rowU, rowB, nullptr, 0, nq);
-#pragma unroll
-        for (int k = 0; k < TT / 4; ++k) {
-            ScanGroup<NS, false> next;
-            if (k + 1 < TT / 4) next.template load<NP>(rowD, rowU, rowB, nullptr, k + 1, nq);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
-                    if (MIX && j) ex[4 * k + i][j] = nq * NS + j < a.N ? ex[4 * k + i][j] : 0.f;
+                for (int i = 0; i < F; ++i) {
+                    const float sg = fast_sigmoid(z4[i]);
+                    Z4[i] = G4[i] * (sg * fmaf(z4[i], 1.f - sg, 1.f));
+                    G4[i] = G4[i] * (z4[i] * sg);
                 }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < F; ++i) tile_skip = fmaf(G4[i], u4[i], tile_skip);
+            dskip += tile_skip;
+            store_pack<float, F>(sD + sch * LD + sq * F, D4);
+            store_pack<float, F>(sU + sch * LD + sq * F, U4);
+            store_pack<float, F>(sG + sch * LD + sq * F, G4);
+            store_pack<float, F>(keep[0].v, D4);
+            store_pack<float, F>(keep[256].v, u4);
+            store_pack<float, F>(keep[512].v, S4);
+            store_pack<float, F>(keep[768].v, G4);
+            store_pack<float, F>(keep[1024].v, Z4);
+            float h[NS];
 #pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    h[j] = fmaf(ex[4 * k + i][j], h[j], at(gr.U, i) * gr.B[i].v[j]);
-                    if (MIX && j) h[j] = nq * NS + j < a.N ? h[j] : 0.f;
-                    hs[4 * k + i][j] = h[j];
+            for (int j = 0; j < NS; ++j) h[j] = rh[j];
+            wave_handover();
+            if (t0 - TT >= p0) fetch(len - t0 + TT);
+            const float *rowB = bc0 + buf * bc_buf, *rowC = rowB + bc_c;
+            float *outD = sD + ch * LD, *outU = outD + L::rows, *outG = outU + L::rows;       // where the sums over the channel's states go
+            float ex[TT][NS], hs[TT][NS], h0[NS];                    // hs[t]: the state behind frame t
+#pragma unroll
+            for (int j = 0; j < NS; ++j) h0[j] = h[j];
+            ScanGroup<NS, false> gr;
+            gr.template load<NP>(rowD, rowU, rowB, nullptr, 0, nq);
+#pragma unroll
+            for (int k = 0; k < TT / 4; ++k) {
+                ScanGroup<NS, false> next;
+                if (k + 1 < TT / 4) next.template load<NP>(rowD, rowU, rowB, nullptr, k + 1, nq);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        ex[4 * k + i][j] = __builtin_amdgcn_exp2f(at(gr.D, i) * A2[j]);
+                        if (MIX && j) ex[4 * k + i][j] = nq * NS + j < a.N ? ex[4 * k + i][j] : 0.f;
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        h[j] = fmaf(ex[4 * k + i][j], h[j], at(gr.U, i) * gr.B[i].v[j]);
+                        if (MIX && j) h[j] = nq * NS + j < a.N ? h[j] : 0.f;
+                        hs[4 * k + i][j] = h[j];
+                    }
+                if (k + 1 < TT / 4) gr = next;
+            }
+            float dat[NS] = {};
+#pragma unroll
+            for (int k = TT / 4 - 1; k >= 0; --k) {
+                ScanGroup<NS, true> gb;
+                gb.template load<NP>(rowD, rowU, rowB, rowC, k, nq);
+                const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
+                __builtin_amdgcn_sched_barrier(0);
+                float o12[12];                                       // (k, b, y) of four frames
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    const int s = 4 * k + i;
+                    const float dt = at(gb.D, i), dui = at(gb.U, i), gi = at(g4, i);
+                    float vB[NS], vC[NS], v[NS / 2];
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        float rj = fmaf(gb.Cv[i].v[j], gi, r[j]);
+                        if (MIX && j) rj = nq * NS + j < a.N ? rj : 0.f;
+                        const float hj = hs[s][j];
+                        r[j] = rj * ex[s][j];
+                        const float rq = r[j] * (s ? hs[s ? s - 1 : 0][j] : h0[j]);
+                        o12[2 + 3 * i] = j ? fmaf(gb.Cv[i].v[j], hj, o12[2 + 3 * i]) : gb.Cv[i].v[j] * hj;
+                        o12[1 + 3 * i] = j ? fmaf(gb.B[i].v[j], rj, o12[1 + 3 * i]) : gb.B[i].v[j] * rj;
+                        o12[0 + 3 * i] = j ? fmaf(A[j], rq, o12[0 + 3 * i]) : A[j] * rq;
+                        dat[j] = fmaf(dt, rq, dat[j]);
+                        vB[j] = rj * dui;
+                        vC[j] = gi * hj;
+                    }
+                    channel_sums<LN, NS>(vB, vC, v);
+                    float* o = sP + (wave * TT + s) * 2 * NP + (lane >> 5) * NP + nq * NS + ((lane >> 4) & 1) * (NS / 2);
+#pragma unroll
+                    for (int j = 0; j < NS / 2; ++j) o[j] = v[j];
                 }
-            if (k + 1 < TT / 4) gr = next;
-        }
-        float dat[NS] = {};
+                lanes_sum4<LN, 3>(o12);
+                float ko[W], bo[W], yo[W];
 #pragma unroll
-        for (int k = TT / 4 - 1; k >= 0; --k) {
-            ScanGroup<NS, true> gb;
-            gb.template load<NP>(rowD, rowU, rowB, rowC, k, nq);
-            const float4 g4 = *reinterpret_cast<const float4*>(rowG + 4 * k);
-            __builtin_amdgcn_sched_barrier(0);
-            float o12[12];                                       // (k, b, y) of four frames
-#pragma unroll
-            for (int i = 3; i >= 0; --i) {
-                const int s = 4 * k + i;
-                const float dt = at(gb.D, i), dui = at(gb.U, i), gi = at(g4, i);
-                float vB[NS], vC[NS], v[NS / 2];
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    float rj = fmaf(gb.Cv[i].v[j], gi, r[j]);
-                    if (MIX && j) rj = nq * NS + j < a.N ? rj : 0.f;
-                    const float hj = hs[s][j];
-                    r[j] = rj * ex[s][j];
-                    const float rq = r[j] * (s ? hs[s ? s - 1 : 0][j] : h0[j]);
-                    o12[2 + 3 * i] = j ? fmaf(gb.Cv[i].v[j], hj, o12[2 + 3 * i]) : gb.Cv[i].v[j] * hj;
-                    o12[1 + 3 * i] = j ? fmaf(gb.B[i].v[j], rj, o12[1 + 3 * i]) : gb.B[i].v[j] * rj;
-                    o12[0 + 3 * i] = j ? fmaf(A[j], rq, o12[0 + 3 * i]) : A[j] * rq;
-                    dat[j] = fmaf(dt, rq, dat[j]);
-                    vB[j] = rj * dui;
-                    vC[j] = gi * hj;
+                for (int i = 0; i < W; ++i) {
+                    ko[i] = o12[3 * i];
+                    bo[i] = o12[1 + 3 * i];
+                    yo[i] = o12[2 + 3 * i];
                 }
-                channel_sums<LN, NS>(vB, vC, v);
-                float* o = sP + (wave * TT + s) * 2 * NP + (lane >> 5) * NP + nq * NS + ((lane >> 4) & 1) * (NS / 2);
-#pragma unroll
-                for (int j = 0; j < NS / 2; ++j) o[j] = v[j];
+                arrived(ko);
+                arrived(bo);
+                arrived(yo);
+                if (nq % 4 == 0) {                                   // the channel's lanes have read these four frames
+                    const int at_ = 4 * k + nq / 4 * W;
+                    store_pack<float, W>(outD + at_, ko);
+                    store_pack<float, W>(outU + at_, bo);
+                    store_pack<float, W>(outG + at_, yo);
+                }
             }
-            lanes_sum4<LN, 3>(o12);
-            float ko[W], bo[W], yo[W];
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                ko[i] = o12[3 * i];
-                bo[i] = o12[1 + 3 * i];
-                yo[i] = o12[2 + 3 * i];
+            for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (a tile's sum first, 32 tiles in float, the rest in double)
+            if (t0 - TT >= p0) {                                     // B and C are the block's: the next tile's go where the last one's were
+                ob.put(lds_bc + (buf ^ 1) * 2 * L::bc, rb);
+                oc.put(lds_bc + (buf ^ 1) * 2 * L::bc + L::bc, rc);
             }
-            arrived(ko);
-            arrived(bo);
-            arrived(yo);
-            if (nq % 4 == 0) {                                   // the channel's lanes have read these four frames
-                const int at_ = 4 * k + nq / 4 * W;
-                store_pack<float, W>(outD + at_, ko);
-                store_pack<float, W>(outU + at_, bo);
-                store_pack<float, W>(outG + at_, yo);
+            __syncthreads();
+            const Pack<float, F> kk = *reinterpret_cast<const Pack<float, F>*>(sD + sch * LD + sq * F), bb = *reinterpret_cast<const Pack<float, F>*>(sU + sch * LD + sq * F);
+            const Pack<float, F> yy = *reinterpret_cast<const Pack<float, F>*>(sG + sch * LD + sq * F);
+            const Pack<float, F> kD = keep[0], ku = keep[256], kS = keep[512], kG = keep[768], kZ = keep[1024];
+            float tile_bias = 0.f, xu[F], xe[F], xz[F];
+#pragma unroll
+            for (int i = 0; i < F; ++i) {
+                xe[i] = fmaf(ku.v[i], bb.v[i], kk.v[i]) * kS.v[i];
+                xu[i] = fmaf(masked(kG.v[i], skip_mask), skip, kD.v[i] * bb.v[i]);
+                xz[i] = kZ.v[i] * fmaf(skip, masked(ku.v[i], skip_mask), yy.v[i]);
+                tile_bias += sq * F + i < len - t0 ? xe[i] : 0.f;
             }
+            dbias += tile_bias;
+            float v[NP2];
+#pragma unroll
+            for (int k = 0; k < NP2; ++k) {
+                const int i = tid + 256 * k;
+                v[k] = (sP[i] + sP[TT * 2 * NP + i]) + (sP[2 * TT * 2 * NP + i] + sP[3 * TT * 2 * NP + i]);
+            }
+            auto write = [&](auto full, int left) __attribute__((always_inline)) {
+                oo.template store<full()>(rows_at(du), sq, left, xu);
+                oo.template store<full()>(rows_at(de), sq, left, xe);
+                ow.template store<full()>(rows_at(dz), sq, left, xz);
+#pragma unroll
+                for (int k = 0; k < NP2; ++k) row_store<float>(v[k], rows_at(bc), full() || (tid + 256 * k) / (2 * NP) < left ? op[k] : SC_OUT, 0);
+            };
+            if (len - t0 >= TT) write(std::true_type(), TT);
+            else write(std::false_type(), len - t0);
+            du += adv * row; de += adv * row; dz += adv * a.dzt; bc += adv * a.B * 2 * NP;
+            if (L::parts == 1) __syncthreads();
         }
+        if (a.acc && t0 >= p0) {                                     // long runs: what has been added up so far moves to the thread's doubles
+            double* acc = a.acc + ((((long long)c * a.B + b) * gridDim.x + blk.x) * (NS + 2)) * 256 + here(tid);
+            auto move = [&](int k, float& v) {
+                acc[k * 256] = (flushed ? acc[k * 256] : 0.) + (double)v;
+                v = 0.f;
+            };
 #pragma unroll
-        for (int j = 0; j < NS; ++j) da[j] += dat[j];            // (a tile's sum first, 32 tiles in float, the rest in double)
-        if (t0 - TT >= p0) {                                     // B and C are the block's: the next tile's go where the last one's were
-            ob.put(lds_bc + (buf ^ 1) * 2 * L::bc, rb);
-            oc.put(lds_bc + (buf ^ 1) * 2 * L::bc + L::bc, rc);
+            for (int j = 0; j < NS; ++j) move(j, da[j]);
+            move(NS, dskip);
+            move(NS + 1, dbias);
+            flushed = true;
         }
-        __syncthreads();
-        const Pack<float, F> kk = *reinterpret_cast<const Pack<float, F>*>(sD + sch * LD + sq * F), bb = *reinterpret_cast<const Pack<float, F>*>(sU + sch * LD + sq * F);
-        const Pack<float, F> yy = *reinterpret_cast<const Pack<float, F>*>(sG + sch * LD + sq * F);
-        const Pack<float, F> kD = keep[0], ku = keep[256], kS = keep[512], kG = keep[768], kZ = keep[1024];
-        float tile_bias = 0.f, xu[F], xe[F], xz[F];
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            xe[i] = fmaf(ku.v[i], bb.v[i], kk.v[i]) * kS.v[i];
-            xu[i] = fmaf(masked(kG.v[i], skip_mask), skip, kD.v[i] * bb.v[i]);
-            xz[i] = kZ.v[i] * fmaf(skip, masked(ku.v[i], skip_mask), yy.v[i]);
-            tile_bias += sq * F + i < len - t0 ? xe[i] : 0.f;
-        }
-        dbias += tile_bias;
-        float v[NP2];
-#pragma unroll
-        for (int k = 0; k < NP2; ++k) {
-            const int i = tid + 256 * k;
-            v[k] = (sP[i] + sP[TT * 2 * NP + i]) + (sP[2 * TT * 2 * NP + i] + sP[3 * TT * 2 * NP + i]);
-        }
-        auto write = [&](auto full, int left) __attribute__((always_inline)) {
-            oo.template store<full()>(rows_at(du), sq, left, xu);
-            oo.template store<full()>(rows_at(de), sq, left, xe);
-            ow.template store<full()>(rows_at(dz), sq, left, xz);
-#pragma unroll
-            for (int k = 0; k < NP2; ++k) row_store<float>(v[k], rows_at(bc), full() || (tid + 256 * k) / (2 * NP) < left ? op[k] : SC_OUT, 0);
-        };
-        if (len - t0 >= TT) write(std::true_type(), TT);
-        else write(std::false_type(), len - t0);
-        du += adv * row; de += adv * row; dz += adv * a.dzt; bc += adv * a.B * 2 * NP;
-        if (L::parts == 1) __syncthreads();
-    }
-    if (a.acc && t0 >= p0) {                                     // long runs: what has been added up so far moves to the thread's doubles
-        double* acc = a.acc + ((((long long)c * a.B + b) * gridDim.x + blk.x) * (NS + 2)) * 256 + here(tid);
-        auto move = [&](int k, float& v) {
-            acc[k * 256] = (flushed ? acc[k * 256] : 0.) + (double)v;
-            v = 0.f;
-        };
-#pragma unroll
-        for (int j = 0; j < NS; ++j) move(j, da[j]);
-        move(NS, dskip);
-        move(NS + 1, dbias);
-        flushed = true;
-    }
     }
     if (a.dh0 && d < a.D && c == 0) store_states<NS>(a.dh0 + ((long long)b * a.D + d) * a.N, nq * NS, a.N, r);
     if (!a.sums) return;
