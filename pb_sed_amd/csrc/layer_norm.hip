@@ -4,8 +4,9 @@
 // A row lives in the registers of LPR lanes (E elements each) between its one load and its one store: the variance is the mean of
 // squared differences from the mean (two sweeps over registers, nothing cancels), and memory sees every tensor once.  Rows wider than
 // 256 x 32 elements are re-read from the caches by a looping form.  Blocks walk rows with a grid stride and keep w, b - and in the
-// backward pass their column sums of dy xh and dy - in registers; the sums leave as one row of partials per block, which a second
-// launch adds in a fixed order (no atomics: results are reproducible).
+// backward pass their column sums of dy xh and dy - in registers; the sums leave as one row of partials per block and 256 turns (so that
+// no more than 256 terms are added in float, however many rows there are), which a second launch adds in double in a fixed order (no
+// atomics: results are reproducible).
 //
 // Bound: HBM (forward x in, y out; backward x and dy in, dx out).  Measured: 20011 rows of 1023 bfloat16: forward 18 us (4.6 TB/s, a large
 // copy reaches 4.67), backward 25 us (4.8 TB/s), its weights' sums 4 us; with element loads for the odd width 58 and 75.  16000 rows of
@@ -20,11 +21,13 @@ struct NormArgs {
     const float *w, *b;             // or null (1, 0)
     void* y;                        // forward: y, backward: dx
     float* stats;                   // [rows][2] mean, rstd (forward: or null)
-    float* ws;                      // backward: [grid][2 C] partial sums of dy xh | dy, or null
+    float* ws;                      // backward: [groups][grid][2 C] partial sums of dy xh | dy, or null
     long long xs, dys;              // row strides of x, dy
     int rows, C;
+    int groups;                     // backward: of NORM_TURNS turns
     float eps;
 };
+constexpr int NORM_TURNS = 256;
 
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
@@ -144,8 +147,6 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(NormArgs a) {
     const NormCols<V, LPR, E, TAIL> cols(lane, a.C);
     float w[E], dw[E], db[E];
     cols.weights(a.w, 1.f, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
     const float inv = 1.f / (float)a.C;
     const int step = gridDim.x * RPB;
     int r = blockIdx.x * RPB + sub;
@@ -158,56 +159,61 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(NormArgs a) {
         rst = *reinterpret_cast<const float2*>(a.stats + 2ll * q);
     };
     fetch(r);
-    for (int r0 = blockIdx.x * RPB; r0 < a.rows; r0 += step, r += step) {
-        const bool on = r < a.rows;
-        float x[E], dy[E];
-        const float2 st = rst;
-        cols.values(rx, on, x);
-        cols.values(rg, on, dy);
-        fetch(r + step);
-        float sg = 0.f, sgx = 0.f;
+    int r0 = blockIdx.x * RPB;
+    for (int group = 0; group < a.groups; ++group) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {                               // where a lane has no column dy = 0: nothing is added
-            x[e] = (x[e] - st.x) * st.y;
-            dw[e] = fmaf(dy[e], x[e], dw[e]);
-            db[e] += dy[e];
-            dy[e] *= w[e];
-            const float g = dy[e] * cols.own(e);
-            sg += g;
-            sgx = fmaf(g, x[e], sgx);
-        }
-        const float mg = row_sum<LPR>(sg, red) * inv, mgx = row_sum<LPR>(sgx, red) * inv;
+        for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+        for (int turn = 0; turn < NORM_TURNS && r0 < a.rows; ++turn, r0 += step, r += step) {
+            const bool on = r < a.rows;
+            float x[E], dy[E];
+            const float2 st = rst;
+            cols.values(rx, on, x);
+            cols.values(rg, on, dy);
+            fetch(r + step);
+            float sg = 0.f, sgx = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) dy[e] = st.y * (dy[e] - mg - x[e] * mgx);
-        if (on) cols.store(static_cast<S*>(a.y) + (long long)r * a.C, dy);
-    }
-    if (!a.ws) return;
-    // the RPB rows side by side meet in LDS, vector after vector; lanes of sub 0 write the block's partials
-    float* out = a.ws + (long long)blockIdx.x * 2 * a.C;
-#pragma unroll
-    for (int k = 0; k < E / V; ++k) {
-        if constexpr (RPB > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                part[((sub * V + j) * 2) * LPR + lane] = dw[k * V + j];
-                part[((sub * V + j) * 2 + 1) * LPR + lane] = db[k * V + j];
+            for (int e = 0; e < E; ++e) {                               // where a lane has no column dy = 0: nothing is added
+                x[e] = (x[e] - st.x) * st.y;
+                dw[e] = fmaf(dy[e], x[e], dw[e]);
+                db[e] += dy[e];
+                dy[e] *= w[e];
+                const float g = dy[e] * cols.own(e);
+                sg += g;
+                sgx = fmaf(g, x[e], sgx);
             }
-            __syncthreads();
+            const float mg = row_sum<LPR>(sg, red) * inv, mgx = row_sum<LPR>(sgx, red) * inv;
+#pragma unroll
+            for (int e = 0; e < E; ++e) dy[e] = st.y * (dy[e] - mg - x[e] * mgx);
+            if (on) cols.store(static_cast<S*>(a.y) + (long long)r * a.C, dy);
         }
-        if (sub == 0 && cols.c[k] >= 0)
+        if (!a.ws) continue;
+        // the RPB rows side by side meet in LDS, vector after vector; lanes of sub 0 write the block's partials
+        float* out = a.ws + ((long long)group * gridDim.x + blockIdx.x) * 2 * a.C;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float s0 = dw[k * V + j], s1 = db[k * V + j];
+        for (int k = 0; k < E / V; ++k) {
+            if constexpr (RPB > 1) {
+                __syncthreads();
 #pragma unroll
-                for (int q = 1; q < RPB; ++q) {
-                    s0 += part[((q * V + j) * 2) * LPR + lane];
-                    s1 += part[((q * V + j) * 2 + 1) * LPR + lane];
+                for (int j = 0; j < V; ++j) {
+                    part[((sub * V + j) * 2) * LPR + lane] = dw[k * V + j];
+                    part[((sub * V + j) * 2 + 1) * LPR + lane] = db[k * V + j];
                 }
-                // (a column that two lanes have: both hold the same sums)
-                out[cols.c[k] + j] = s0;
-                out[a.C + cols.c[k] + j] = s1;
+                __syncthreads();
             }
+            if (sub == 0 && cols.c[k] >= 0)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float s0 = dw[k * V + j], s1 = db[k * V + j];
+#pragma unroll
+                    for (int q = 1; q < RPB; ++q) {
+                        s0 += part[((q * V + j) * 2) * LPR + lane];
+                        s1 += part[((q * V + j) * 2 + 1) * LPR + lane];
+                    }
+                    // (a column that two lanes have: both hold the same sums)
+                    out[cols.c[k] + j] = s0;
+                    out[a.C + cols.c[k] + j] = s1;
+                }
+        }
     }
 }
 
@@ -219,12 +225,12 @@ __global__ __launch_bounds__(256) void layer_norm_wide_fwd_kernel(NormArgs a) {
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const S* x = static_cast<const S*>(a.x) + r * a.xs;
         S* y = static_cast<S*>(a.y) + (long long)r * a.C;
-        float s = 0.f;
-        for (int c = threadIdx.x; c < a.C; c += 256) s += (float)x[c];
-        const float mean = row_sum<256>(s, red) * inv;
-        s = 0.f;
-        for (int c = threadIdx.x; c < a.C; c += 256) { const float d = (float)x[c] - mean; s = fmaf(d, d, s); }
-        const float rstd = 1.f / sqrtf(fmaf(row_sum<256>(s, red), inv, a.eps));
+        double s = 0.;                                              // (up to 65536 terms of a thread)
+        for (int c = threadIdx.x; c < a.C; c += 256) s += (double)x[c];
+        const float mean = row_sum<256>((float)s, red) * inv;
+        s = 0.;
+        for (int c = threadIdx.x; c < a.C; c += 256) { const float d = (float)x[c] - mean; s += (double)(d * d); }
+        const float rstd = 1.f / sqrtf(fmaf(row_sum<256>((float)s, red), inv, a.eps));
         for (int c = threadIdx.x; c < a.C; c += 256)
             y[c] = (S)fmaf(((float)x[c] - mean) * rstd, a.w ? a.w[c] : 1.f, a.b ? a.b[c] : 0.f);
         if (a.stats && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + 2ll * r) = make_float2(mean, rstd);
@@ -235,25 +241,30 @@ __global__ __launch_bounds__(256) void layer_norm_wide_bwd_kernel(NormArgs a) {
     __shared__ float red[4];
     const float inv = 1.f / (float)a.C;
     float* out = a.ws ? a.ws + (long long)blockIdx.x * 2 * a.C : nullptr;
-    bool first = true;
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x, first = false) {
+    int turn = 0;
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x, ++turn) {
+        const bool first = turn % NORM_TURNS == 0;
+        if (first && turn && out) out += 2ll * gridDim.x * a.C;
         const S *x = static_cast<const S*>(a.x) + r * a.xs, *dy = static_cast<const S*>(a.dy) + r * a.dys;
         S* dx = static_cast<S*>(a.y) + (long long)r * a.C;
         const float mean = a.stats[2ll * r], rstd = a.stats[2ll * r + 1];
-        float sg = 0.f, sgx = 0.f;
+        double sg = 0., sgx = 0.;
         for (int c = threadIdx.x; c < a.C; c += 256) {
             const float g = (float)dy[c], xh = ((float)x[c] - mean) * rstd, gw = g * (a.w ? a.w[c] : 1.f);
-            sg += gw;
-            sgx = fmaf(gw, xh, sgx);
+            sg += (double)gw;
+            sgx += (double)(gw * xh);
             if (out) {                                              // a column belongs to one thread: its partials add up in memory
                 out[c] = first ? g * xh : fmaf(g, xh, out[c]);
                 out[a.C + c] = first ? g : out[a.C + c] + g;
             }
         }
-        const float mg = row_sum<256>(sg, red) * inv, mgx = row_sum<256>(sgx, red) * inv;
+        const float mg = row_sum<256>((float)sg, red) * inv, mgx = row_sum<256>((float)sgx, red) * inv;
         for (int c = threadIdx.x; c < a.C; c += 256)
             dx[c] = (S)(rstd * ((float)dy[c] * (a.w ? a.w[c] : 1.f) - mg - ((float)x[c] - mean) * rstd * mgx));
     }
+    // the last group of a block that has one turn less than its neighbours
+    if (out && turn <= (a.groups - 1) * NORM_TURNS)
+        for (int c = threadIdx.x; c < 2 * a.C; c += 256) out[2ll * gridDim.x * a.C + c] = 0.f;
 }
 
 __global__ __launch_bounds__(SUM_THREADS) void norm_sum_kernel(const float* ws, int P, long W, SumSegs sg) {
@@ -277,6 +288,13 @@ static int norm_grid(int rows, int C, bool bwd) {
     if (C <= 8192) norm_shape(C, &lpr, &e);
     const int rpb = 256 / lpr, need = (rows + rpb - 1) / rpb, most = device_cus() * (bwd ? (e >= 32 ? 1 : e == 16 ? 2 : 4) : (e >= 32 ? 2 : e == 16 ? 4 : 8));
     return need < most ? need : most;
+}
+
+static int norm_groups(int rows, int C, int grid) {
+    int lpr = 256, e = 32;
+    if (C <= 8192) norm_shape(C, &lpr, &e);
+    const long long turn = (long long)grid * (256 / lpr);
+    return (int)((rows + turn * NORM_TURNS - 1) / (turn * NORM_TURNS));
 }
 
 template <class S, int V, int LPR, int E>
@@ -343,7 +361,8 @@ extern "C" int pbsed_layer_norm_fwd(const void* x, const float* w, const float* 
 
 extern "C" long long pbsed_layer_norm_workspace(long long rows, long long C) {
     if (rows < 1 || rows > 0x3fffffff || C < 1 || C > (1 << 24)) return 0;
-    return (long long)norm_grid((int)rows, (int)C, true) * 2 * C;
+    const int grid = norm_grid((int)rows, (int)C, true);
+    return (long long)grid * norm_groups((int)rows, (int)C, grid) * 2 * C;
 }
 
 extern "C" int pbsed_layer_norm_bwd(const void* dy, const void* x, const float* w, const float* stats, void* dx, float* dw, float* db,
@@ -364,10 +383,12 @@ extern "C" int pbsed_layer_norm_bwd(const void* dy, const void* x, const float* 
     NormArgs a{};
     a.x = x; a.dy = dy; a.w = w; a.y = dx; a.stats = const_cast<float*>(stats); a.ws = sums ? ws : nullptr;
     a.rows = (int)rows; a.C = (int)C; a.xs = x_stride; a.dys = dy_stride;
+    const int grid = norm_grid(a.rows, a.C, true);
+    a.groups = norm_groups(a.rows, a.C, grid);
     int rc = PBSED_OK;
     PBSED_ELEM(dtype, rc = norm_launch<S>(a, true, (hipStream_t)stream));
     if (rc || !sums) return rc;
     const SumSegs sg{{dw, db, nullptr}, {(int)C, (int)(2 * C), (int)(2 * C)}};
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(SUM_THREADS), 0, (hipStream_t)stream, ws, norm_grid(a.rows, a.C, true), (long)(2 * C), sg);
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(SUM_THREADS), 0, (hipStream_t)stream, ws, grid * a.groups, (long)(2 * C), sg);
     return check_launch("layer_norm_bwd sums");
 }

@@ -266,3 +266,23 @@ def test_sums_of_long_uncut_scans_keep_their_digits(dev):             # noqa: F8
         want -= r * decay[f] * past[f] * step[f]
         r = r * decay[f]
     check(da, b * want, b * want.abs(), k + 2 * 42, 'da_log')
+
+
+@pytest.mark.parametrize('c,rows', [(9, 140_000), (300, 10_000), (9000, 2500)])      # more than 256 turns of eight CUs
+def test_sums_of_many_rows_keep_their_digits(dev, c, rows):           # noqa: F811
+    """Layer norm's weight gradients over rows whose terms have one sign: a block adds at most 256 turns in float."""
+    from pb_sed_amd import ops
+    if dev != 'cpu':
+        rows = {9: 40_000_000, 300: 10_000_000, 9000: 500_000}[c]     # thousands of turns of 256 CUs
+    row = normal(torch.Generator().manual_seed(c), 1, c).float()
+    x = row.to(dev).expand(rows, c).contiguous()
+    dy = torch.full((rows, c), 4 / 3, device=dev)                     # (as above)
+    _, stats = ops.layer_norm_fwd(x, save=True)
+    dw, db = torch.zeros(c, device=dev), torch.zeros(c, device=dev)
+    ops.layer_norm_bwd(dy, x, None, stats, dweight=dw, dbias=db)
+    want = rows * dy[0].double().cpu()
+    k = 256 + 16 + 2                                                  # turns, rows of a block side by side, two conversions
+    check(db, want, want, k, 'dbias')
+    mean, rstd = stats[0].double().cpu()
+    xh = (row[0].double() - mean) * rstd                              # (two roundings of a term: the difference and the product)
+    check(dw, want * xh, (want * xh).abs(), k + 3, 'dweight')
