@@ -549,11 +549,13 @@ def _wgrad_job(jobs, dg, x, shift, dw, db):
 def dropout_state(wrapper, device):
     """The (seed, step) of a training pass's masks between the layers of ``wrapper``, on the device.  The seed comes from torch's CPU
     generator at the first pass (torch.manual_seed governs it; ranks that shall draw different masks seed it differently), the step
-    counts the passes."""
-    if wrapper.dropout_rng is None or wrapper.dropout_rng.device != device:
+    counts the passes; a trainer checkpoint carries both."""
+    rng = wrapper.dropout_rng
+    if rng is None or rng.device != device:
         if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
             raise RuntimeError('the first training pass of a GRU with dropout copies its seed to the device: run one before a graph is captured')
-        wrapper.dropout_rng = ops.host_to_device(np.array([torch.randint(1 << 62, ()).item(), 0]), device, torch.int64)
+        state = [torch.randint(1 << 62, ()).item(), 0] if rng is None else rng.tolist()
+        wrapper.dropout_rng = ops.host_to_device(np.array(state), device, torch.int64)
     now = wrapper.dropout_rng.clone()
     wrapper.dropout_rng[1] += 1
     return now

@@ -476,12 +476,29 @@ class Trainer:
         self._check_flags(0)
 
     # ------------------------------------------------------------------------------------------ checkpoints
-    def state_dict(self):
+    def _dropout_wrappers(self):
+        return {n: m for n, m in self.model.named_modules() if getattr(m, 'dropout', 0.) and hasattr(m, 'dropout_rng')}
+
+    def _dropout_states(self, gather=False):
+        """{GRU module: [[seed, step] of the masks between its layers] per rank} (seed -1: no training pass yet); this rank's alone
+        without ``gather``, which every rank has to call."""
+        wrappers = self._dropout_wrappers()
+        own = [[-1, 0] if m.dropout_rng is None else m.dropout_rng.tolist() for m in wrappers.values()]
+        ranks = [own]
+        if gather and own and dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+            mine = torch.tensor(own, device='cpu' if dist.get_backend() == 'gloo' else self.flat_param.device)
+            parts = [torch.empty_like(mine) for _ in range(dist.get_world_size())]
+            dist.all_gather(parts, mine)
+            ranks = [p.tolist() for p in parts]
+        return {n: [r[i] for r in ranks] for i, n in enumerate(wrappers)}
+
+    def state_dict(self, dropout=None):
         """What a resume needs, in the layout of a padertorch trainer checkpoint (``{'model', 'iteration', 'epoch',
         'optimizer'}``; pb_sed/experiments/weak_label_crnn/inference.py:407-413 reads ``ckpt['model']`` through
         ``Model.from_storage_dir``): the model's state_dict under the reference's parameter / buffer names and Adam's state
         as a ``torch.optim.Adam`` state_dict over ``model.parameters()`` in order (exp_avg / exp_avg_sq views of the flat moment
         buffers, ``step`` = the iteration), so that ``torch.optim.Adam.load_state_dict`` can take the 'optimizer' entry as it is.
+        'rnn_dropout' holds what the masks between GRU layers are drawn from (``_dropout_states``; ``dropout``: the ranks' together).
         ('hooks', the per-hook state padertorch's trainer also writes, is carried as an empty dict: this trainer has no hooks with
         state.  Whether padertorch's ``Trainer.load_checkpoint`` accepts the file is NOT verified - padertorch is not installed.)"""
         self.finish()
@@ -494,7 +511,8 @@ class Trainer:
                  'params': list(range(len(params)))}
         return {'model': {k: v.detach().clone().cpu() for k, v in self.model.state_dict().items()},
                 'iteration': self.iteration, 'epoch': getattr(self, 'epoch', 0),
-                'optimizer': {'state': state if self.iteration else {}, 'param_groups': [group]}, 'hooks': {}}
+                'optimizer': {'state': state if self.iteration else {}, 'param_groups': [group]}, 'hooks': {},
+                'rnn_dropout': self._dropout_states() if dropout is None else dropout}
 
     def load_state_dict(self, ckpt):
         """Resume from ``state_dict()`` output or from a padertorch trainer checkpoint of the same model (Adam state keyed by
@@ -512,6 +530,11 @@ class Trainer:
             self.m[sl].copy_(st['exp_avg'].reshape(-1))
             self.v[sl].copy_(st['exp_avg_sq'].reshape(-1))
             self.iteration = max(self.iteration, int(float(st.get('step', self.iteration))))
+        rank = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+        for name, m in self._dropout_wrappers().items():             # every rank goes on with its own masks; a new rank draws a seed
+            states = (ckpt.get('rnn_dropout') or {}).get(name) or []
+            if rank < len(states) and states[rank][0] >= 0:
+                m.dropout_rng = torch.tensor(states[rank])            # (moves to the device at the next pass)
         for g in opt.get('param_groups') or []:
             self.lr, self.betas, self.eps = g.get('lr', self.lr), tuple(g.get('betas', self.betas)), g.get('eps', self.eps)
         if self.flat_param.is_cuda:
@@ -524,10 +547,11 @@ class Trainer:
         rank 0 writes.  Returns the path."""
         import os
         self.sync_buffers()
+        dropout = self._dropout_states(gather=True)
         path = os.path.join(storage_dir, 'checkpoints', name or f'ckpt_{self.iteration}.pth')
         if not (dist.is_available() and dist.is_initialized()) or dist.get_rank() == 0:
             os.makedirs(os.path.dirname(path), exist_ok=True)
-            torch.save(self.state_dict(), path)
+            torch.save(self.state_dict(dropout), path)
         return path
 
     def load_checkpoint(self, path, map_location='cpu', trusted_pickle=False):
