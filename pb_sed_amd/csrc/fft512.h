@@ -2,6 +2,8 @@
 // per lane of a 64-wide wave; the passes and the real-FFT-1024 unpacking live next to their LDS indexing in logmel.hip).
 // Which products are rounded and which are part of a fused multiply-add is written out: left to the compiler, every unrolled copy of a
 // butterfly rounds in its own way, which changes with vector forms and flags.
+// (The forms are equally good: against a float64 transform of 512 normal numbers the relative rms error is 1.02e-7 as written, 1.00 .. 1.07e-7
+// in eleven other consistent choices.  Their features differ in the last bits, so that a max-pool or ReLU branch behind them can tip.)
 #pragma once
 #ifdef __HIPCC__
 #define PBSED_HD __host__ __device__ __forceinline__
