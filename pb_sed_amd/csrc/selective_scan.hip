@@ -219,7 +219,7 @@ __global__ __launch_bounds__(1024) void scan_runs_kernel(ScanArgs a, int NP, int
 // Steps below zero (softplus = 0 only) have factors above one, and over a run both their product and the run's end state from zero can leave
 // float while the state itself does not (it may be 0 there, tiny, or cancelled by the run's first frames).  Without softplus the states in
 // front of the runs are therefore left by this kernel whatever their number, one run after the other: the factor meets the state with its
-// exponent apart, and a run whose result is not finite all the same is walked frame by frame from the state in front of it, as the uncut
+// exponent apart, and a run that takes a finite state to one that is not is walked frame by frame from the state in front of it, as the uncut
 // scan does.  A lane owns one state.
 __device__ __forceinline__ float carried(float x, float e) {       // exp2(e) x
     const float whole = floorf(e);
@@ -271,7 +271,8 @@ __global__ __launch_bounds__(64) void scan_runs_careful_kernel(ScanArgs a, int N
             if (k < a.nrun) a.runs[(long long)c * M + m] = x;
             if (k < a.nrun - 1) {
                 const float next = carried(x, dt[i] * A2) + s[i];
-                x = fabsf(next) <= 3.402823466e38f || x != x || !real ? next : walk(c, x);
+                const bool finite = fabsf(next) <= 3.402823466e38f, was = fabsf(x) <= 3.402823466e38f;
+                x = finite || !was || !real ? next : walk(c, x);   // (what is not finite in front of a run is not finite behind it)
             }
         }
     }

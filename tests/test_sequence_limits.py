@@ -94,6 +94,21 @@ def test_growing_scans_do_not_depend_on_the_cut(dev):                 # noqa: F8
     check(h, want['state_out'], want['major']['state_out'], 94, 'state, frame by frame')
 
 
+def test_growing_scans_that_leave_float32_stay_outside(dev):          # noqa: F811
+    """Driven from the first frame: finite up to float32's range as in the formula, and not finite in any run behind that."""
+    from pb_sed_amd import ops
+    t, d, n = 400, 5, 4
+    v = growing(t, d, n)
+    v['u'][:20] = 1.
+    v['b'].abs_(), v['c'].abs_().add_(.5)
+    want = ref.scan(*(v[k].double() for k in ('u', 'delta', 'a_log', 'b', 'c')), softplus=False)
+    y, state = scan_forward(ops, up(v, dev), softplus=False)
+    inside = want['y'].abs() < 1e37                                   # (the states too: c >= 0.5)
+    assert inside.any() and not inside.all() and not torch.isfinite(y.cpu()[want['y'].abs() > 1e39]).any()
+    check(y.cpu()[inside], want['y'][inside], want['major']['y'][inside], 94, 'y')
+    assert not torch.isfinite(state).any()
+
+
 # ------------------------------------------------------------------------------------------------ infinities beside padding
 # States are padded to 8, 16, 32 or 64 and channels to a block; an infinity that the formula keeps must not meet their zeros.
 def same(got, want, what):
