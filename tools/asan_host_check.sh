@@ -13,7 +13,7 @@ ASAN=$(ls /opt/rocm/lib/llvm/lib/clang/*/lib/linux/libclang_rt.$RT-x86_64.so 2>/
 [ -n "$ASAN" ] || { echo "no libclang_rt.asan in this image"; exit 77; }
 mkdir -p $W/build
 cd $ROOT/pb_sed_amd/csrc
-FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC $SAN -fno-gpu-sanitize -fno-omit-frame-pointer -Wno-unused-result -Wno-unused-value"
+FLAGS="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC $SAN -fno-gpu-sanitize -fno-omit-frame-pointer -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops"
 pids=()
 for f in api conv conv_bf16 conv_wino conv_winox3 conv_s16 conv1d_pc conv_wgrad gru gru_stack gru_wgrad tm_gemm causal_conv selective_scan layer_norm dropout misc logmel postproc collective; do
   /opt/rocm/bin/hipcc $FLAGS -c $f.hip -o $W/build/$f.o 2> $W/build/$f.err &

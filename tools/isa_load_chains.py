@@ -27,6 +27,7 @@ src = os.path.abspath(args.src)
 with tempfile.TemporaryDirectory() as tmp:
     out = os.path.join(tmp, 'k.s')
     cmd = ['/opt/rocm/bin/hipcc', '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-result', '-Wno-unused-value',
+           '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
            '-S', '--cuda-device-only', src, '-o', out] + [f'-D{d}' for d in args.D]
     r = subprocess.run(cmd, cwd=os.path.dirname(src), capture_output=True, text=True)
     if r.returncode:

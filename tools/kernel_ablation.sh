@@ -9,7 +9,7 @@ cd "$(dirname "$0")/.."
 src=$1; macro=$2; cmd=$3
 mkdir -p gpurun_out/abl
 for d in ${DBGS:-0 1 2 3 8 11}; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Wno-unused-value -D$macro=$d \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops -D$macro=$d \
     -c pb_sed_amd/csrc/$src.hip -o gpurun_out/abl/v$d.o 2>/dev/null &
 done
 wait

@@ -1,7 +1,7 @@
 #!/bin/bash
 # Print VGPR/AGPR/occupancy/spill per kernel of one .hip file:  tools/kernel_resources.sh conv.hip
 cd "$(dirname "$0")/../pb_sed_amd/csrc"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -c "$1" -o /tmp/_kr.o \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops -c "$1" -o /tmp/_kr.o \
   -Rpass-analysis=kernel-resource-usage 2>&1 | \
   grep -E "Function Name|VGPRs:|AGPRs|VGPRs Spill|ScratchSize|Occupancy|LDS Size" | \
   sed -E 's/.*remark: //; s/ \[-Rpass.*//' | paste - - - - - - - | \
