@@ -462,7 +462,7 @@ int pbsed_causal_conv_bwd(const void* dy, const void* x, const float* w, const f
 int pbsed_causal_conv_step(const void* x, const float* w, const float* bias, const void* state, void* state_out, void* y, int B,
                            int D, int K, long long x_stride_b, int silu, int dtype, void* stream);
 /* h_t = exp(D_t A) h_{t-1} + D_t u_t B_t, y_t = (C_t . h_t + skip u_t) silu(z_t) with D_t = softplus(delta_t + delta_bias) (softplus = 0: the
- * sum itself), A = -exp(a_log [D][N]), N <= 64; b, c [T][B][N]; skip, z, delta_bias may be NULL; state / state_out [B][D][N] float or
+ * sum itself, of either sign), A = -exp(a_log [D][N]), N <= 64; b, c [T][B][N]; skip, z, delta_bias may be NULL; state / state_out [B][D][N] float or
  * NULL.  strides (host): frame and clip stride of u, delta, b, c, z.  saved: what the backward pass needs (pbsed_selective_scan_plan
  * gives its size), or NULL.  y [T][B][D] contiguous. */
 int pbsed_selective_scan_plan(int T, int B, int D, int N, int backward, long long* saved_floats /*host*/, long long* ws_floats /*host*/);
