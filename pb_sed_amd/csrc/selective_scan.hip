@@ -665,12 +665,13 @@ __device__ __forceinline__ void channel_sums(const float (&vB)[NS], const float 
 
 // grid (channel blocks, B, runs).  Tiles of 16 frames from the back: the tile's states are recomputed from the saved state in front of
 // it and kept in registers beside the exponentials, then the adjoint runs back over them (r q = r exp(D A) h_{t-1} is the adjoint that
-// moves on times the state before).  What a thread
-// needs again when the tile's sums are known (D, u, sigmoid(raw), g, dy silu'(z) of its frames) waits in its own corner of LDS.  A wave
-// stages its own channels, so that a tile has one barrier (B, C and the sums over the block's channels).
+// moves on times the state before).  What a thread needs again when the tile's sums are known (D, u, sigmoid(raw), g, dy silu'(z) of its
+// frames) waits in its own corner of LDS.  A wave stages its own channels, so that a tile has one barrier (B, C and the sums over the
+// block's channels).
 // Bound: vector instructions - 51 per frame and wave (64 / LN channels) with the staging, of which two are exponentials for the states;
-// they issue in 79 % of the time that two waves per SIMD are resident - and the longest clips' chains, behind whose ends the device runs empty.  Measured (500 frames x 32 clips of falling length x 512
-// channels x 16 states, float, in a trace): forward 53 us, backward 125 us, its sums 8 (with whole sums in every lane the pass took 10 us more).
+// they issue in 79 % of the time that two waves per SIMD are resident - and the longest clips' chains, behind whose ends the device runs
+// empty.  Measured (500 frames x 32 clips of falling length x 512 channels x 16 states, float, in a trace): forward 53 us, backward
+// 125 us, its sums 8 (with whole sums in every lane the pass took 10 us more).
 template <int LN, int NS> struct ScanBwdLds {
     static constexpr int NP = NS * LN, CB = 256 / LN, TT = SC_SAVE, LD = TT + 4, F = CB * TT / 256;
     static constexpr int rows = (CB + 1) * LD, bc = TT * NP, part = 4 * TT * 2 * NP, keep = 5 * 256 * F;
