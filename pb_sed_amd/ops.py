@@ -1582,7 +1582,7 @@ def _scan_plan(dev, t, b, d, n, backward):
 def selective_scan_fwd(u, delta, a_log, b, c, *, d=None, z=None, delta_bias=None, softplus=True, seq_len=None, reverse=False, state=None,
                        want_state=False, save=False):
     """Selective state-space scan: per channel and state  h_t = exp(D_t A) h_{t-1} + D_t u_t b_t,  y_t = (c_t . h_t + d u_t) silu(z_t),
-    D_t = softplus(delta_t + delta_bias) (``softplus=False``: the sum itself), A = -exp(a_log).  u, delta, z [T,B,D]; b, c [T,B,N]; a_log
+    D_t = softplus(delta_t + delta_bias) (``softplus=False``: the sum itself, of either sign), A = -exp(a_log).  u, delta, z [T,B,D]; b, c [T,B,N]; a_log
     float32 [D,N], N <= 64; d, delta_bias [D]; z / d / delta_bias may be None.  ``state`` float32 [B,D,N]: h in front of the first frame.
     Returns (y [T,B,D], state_out [B,D,N] | None, saved | None): ``saved`` (``save=True``) is what ``selective_scan_bwd`` takes."""
     name = 'selective_scan_fwd'
